@@ -401,6 +401,121 @@ int stx_norm_gemv(const void* h, const void* a, const void* w_norm, float eps, c
 int stx_decode_finish(const void* logits, int64_t V, int dtype, float* logits_out, int64_t* token, int64_t* pos,
                       const int64_t* gen_base, int64_t* generated, int64_t max_len, void* workspace, void* stream);
 
+/* ------------------------------------------------------------------ decoding from drafted tokens
+ * No counterpart in the reference, whose host loop decodes one token at a time (src/modeling_skip.py through
+ * transformers' generate).  One step of a speculative decoder around the sparse MLP:
+ *   stx_kv_append (rotates, writes the nodes' keys and values) -> stx_tree_attention -> ... -> stx_verify_draft ->
+ *   stx_kv_keep (the accepted nodes' rows move together).
+ * Lengths, starts, counts, positions, tokens and parents are int64 on the device: nothing is read back and every
+ * entry can be captured in a CUDA graph.
+ *
+ * A draft of sequence b is counts[b] nodes (counts == NULL: all n_tokens); node 0 is the root (the pending token).  Node i
+ * is written to slot start[b] + i of the cache, whatever its depth; its position (for the rotation) is an input.         */
+#define STX_DRAFT_MAX 64 /* nodes of a draft */
+
+/* How a cache holds a row of head_dim values.  The 8-bit forms keep one fp32 scale a row: with a = max |x|,
+ * scale = a / M (M = 127 for int8, 448 for e4m3), code = round-to-nearest-even(x * (M / a)), and the row stands for
+ * code * scale.  A row with a value that is not finite gets the scale NaN and codes 0: it reads back as NaN.  A row whose
+ * scale would be below the smallest normal fp32 number is held as zeros (scale 0).                                       */
+typedef enum { STX_STORE_SAME = 0, STX_STORE_INT8 = 1, STX_STORE_E4M3 = 2 } stx_store;
+
+/* k, v: [n_seq, n_kv_heads, max_len, head_dim] in `store` (STX_STORE_SAME: in dtype), head_dim contiguous, the other
+ * strides in elements and the same for k and v.  k_scale, v_scale: [n_seq, n_kv_heads, max_len] fp32 with contiguous
+ * slots (NULL for STX_STORE_SAME).  dtype: type of the model's activations.                                              */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t seq_stride, head_stride, slot_stride;
+  int64_t scale_seq_stride, scale_head_stride;
+  int64_t max_len;
+  int n_seq, n_kv_heads, head_dim, store, dtype;
+} stx_kv;
+
+/* [n_seq, n_tokens, heads, head_dim], head_dim contiguous, the other strides in elements. */
+typedef struct {
+  void* data;
+  int64_t seq_stride, token_stride, head_stride;
+} stx_heads;
+
+/* Rotary positions: the first rotary_dim values of a head form rotary_dim / 2 pairs, (i, i + rotary_dim / 2) or, interleaved,
+ * (2 i, 2 i + 1); pair i is turned by position * turns[i] full turns and multiplied by factor.  turns: rotary_dim / 2 doubles
+ * on the device.  The angle, its sine and cosine are formed in fp64, so a position of millions is as exact
+ * as the first.                                                                                                           */
+typedef struct {
+  const double* turns;
+  int rotary_dim, interleaved;
+  double factor;
+} stx_rotary;
+
+/* out = x with its rotary pairs turned (inverse != 0: turned back and multiplied by factor, the transposed map and so the
+ * gradient); values behind rotary_dim are copied.  out may be x.  positions [n_seq, n_tokens], row stride
+ * position_stride.  head_dim <= 1024, rotary_dim even and <= head_dim.                                                     */
+int stx_rope(const stx_heads* x, const stx_heads* out, int64_t n_seq, int64_t n_tokens, int heads, int head_dim,
+             const int64_t* positions, int64_t position_stride, const stx_rotary* rotary, int inverse, int dtype, void* stream);
+
+/* Writes token t < counts[b] of sequence b to slot start[b] + t: k rotated (rotary == NULL: as it is) and held in cache->store,
+ * v held in cache->store.  The rotation's result is held in fp32 up to the one rounding of the store.  q (optional,
+ * q->data may be NULL): rotated the same way into q_out in dtype (q_out may be q); rows of tokens t >= counts[b] become zeros
+ * there.  positions NULL: the slot's number.  A slot outside 0..max_len-1 is skipped, and so is a token t >= counts[b]: the
+ * cache's other rows stay as they were.  head_dim <= 256.                                                                  */
+int stx_kv_append(const stx_kv* cache, const stx_heads* k, const stx_heads* v, int64_t n_tokens, const int64_t* start,
+                  const int64_t* counts, const stx_rotary* rotary, const int64_t* positions, int64_t position_stride,
+                  const stx_heads* q, const stx_heads* q_out, int n_heads, void* stream);
+
+/* k_out, v_out [n_seq, n_kv_heads, n, head_dim] contiguous in dtype: the values that slots start[b] .. start[b] + n - 1 stand
+ * for (start NULL: 0); zeros for slots outside 0..max_len-1.                                                               */
+int stx_kv_read(const stx_kv* cache, const int64_t* start, int64_t n, void* k_out, void* v_out, void* stream);
+
+/* Slot start[b] + i takes the row of slot start[b] + path[b, i], for i < counts[b], as if all rows were read before the
+ * first is written; a pair with a slot outside 0..max_len-1 is skipped.  path [n_seq, n_path], row stride path_stride,
+ * n_path <= STX_DRAFT_MAX.  The cache has `layers` layers, layer_stride elements (scale_layer_stride scales) apart, and all
+ * of them are treated the same way in one launch.                                                                          */
+int stx_kv_keep(const stx_kv* cache, int64_t layers, int64_t layer_stride, int64_t scale_layer_stride, const int64_t* start,
+                const int64_t* path, int64_t path_stride, int64_t n_path, const int64_t* counts, void* stream);
+
+/* What each node of a draft sees, from its parents [n_seq, n_tokens] (parent < node; the root has -1): bit j of
+ * masks[b, i] is set when j is i or an ancestor of i, depth[b, i] = number of ancestors (depth may be NULL).  A node whose parent is
+ * not in 0..i-1 sees itself only, at depth 0.  Contiguous, n_tokens <= STX_DRAFT_MAX.                                     */
+int stx_draft_masks(const int64_t* parents, int64_t n_seq, int64_t n_tokens, int64_t* masks, int64_t* depth, void* stream);
+
+/* out[b, i, h] = sum_j p_j v_j with p the soft-max over the visible slots j of scale * q[b, i, h] . k_j; query heads
+ * g * n_heads / n_kv_heads .. read cache head g.  Node i < counts[b] sees slots 0 .. length[b] - 1 and the nodes j < counts[b] of the
+ * draft (slot length[b] + j) whose bit is set in masks[b * mask_stride + i]; masks NULL: j <= i.  Slots from max_len on do
+ * not exist; a length below 0 counts as 0.  A node that sees nothing gets zeros, and so do rows i >= counts[b].  What a masked
+ * slot holds, NaN included, does not matter to the nodes that do not see it.
+ * q, out: [n_seq, n_tokens, n_heads, head_dim] in cache->dtype; n_tokens <= STX_DRAFT_MAX, n_seq <= 1024,
+ * head_dim <= 256 (a multiple of 8; of 16 for the 8-bit stores), n_heads / n_kv_heads <= 64.
+ * workspace: stx_tree_attention_workspace_bytes() bytes of device memory, 16-byte aligned, in any state; it is written and
+ * read by the call only, so calls that may overlap need one each.                                                          */
+int stx_tree_attention_workspace_bytes(int64_t n_tokens, int n_heads, int n_kv_heads, int head_dim, int dtype, size_t* bytes_out);
+int stx_tree_attention(const stx_kv* cache, const stx_heads* q, const stx_heads* out, int64_t n_tokens, int n_heads, float scale,
+                       const int64_t* length, const int64_t* counts, const int64_t* masks, int64_t mask_stride, void* workspace,
+                       void* stream);
+
+/* Walks a draft with the target's choices and gives the accepted nodes and the next token.
+ * tokens [n_seq, n_tokens] (node i's token; tokens[b, 0] is the root's and not looked at).  Results, all int64: path
+ * [n_seq, n_tokens] = the accepted nodes, the root first, -1 behind them; count [n_seq] = their number; next [n_seq] = the token
+ * behind the last of them.  counts[b] <= 0: path -1, count 0, next -1.
+ * target_probs [n_seq, n_tokens, V] fp32, contiguous rows (row i: the target's distribution behind node i), and uniform
+ * [n_seq, n_tokens] fp32 in [0, 1):
+ *   draft_probs == NULL: at the node reached, v, a token is drawn from row v with uniform[b, v]; the walk goes on at v's child
+ *     with that token (the lowest of equal ones), else the token is `next`.  parents NULL: a chain.
+ *   draft_probs [n_seq, n_tokens - 1, V] (a chain; parents must be NULL): row i - 1 is the distribution that node i's token was drawn from.
+ *     Node i is accepted when uniform[b, i] * draft_probs[i - 1][x] < target_probs[i - 1][x]; at the first one refused, `next` is
+ *     drawn from max(target - draft, 0) (the target's row where that is all zeros), behind the last one from the target's row, both
+ *     with uniform[b, 0].  Either way the tokens follow the target's distribution.
+ * Drawing: the first index whose running sum exceeds u times the row's sum, in fp64, so that the result does not depend on the order of
+ * summation but for ties at 1e-15; the last index of positive weight when rounding leaves none.  A row whose sum is not finite or not positive gives -1.
+ * target_tokens [n_seq, n_tokens] int64 instead of target_probs (then uniform and draft_probs are NULL): the token that the target
+ * chooses behind each node (greedy decoding).
+ * V <= STX_VERIFY_MAX_VOCAB, n_tokens <= STX_DRAFT_MAX.                                                                    */
+#define STX_VERIFY_MAX_VOCAB 400000
+int stx_verify_draft(const int64_t* tokens, const int64_t* parents, const float* target_probs, const int64_t* target_tokens,
+                     const float* draft_probs, const float* uniform, const int64_t* counts, int64_t n_seq, int64_t n_tokens,
+                     int64_t V, int64_t* path, int64_t* count, int64_t* next, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,8 @@ README "sparse_mlp_forward(x, concat_w, active_down_w, down_buf, combined_buf, a
   approx_topk_threshold  torch.ops.sparse_mlp.approx_topk_threshold
 
 plus the host-side mirror of the three hot functions of src/modeling_skip.py
-(FastLoRAProjection, SkipMLP, compute_binary_mask) and the fused layer/stack objects.
+(FastLoRAProjection, SkipMLP, compute_binary_mask), the fused layer/stack objects, and what decoding from drafted
+tokens needs around them (RotaryPositions, KVCache, draft_masks, tree_attention, verify_draft).
 
 Everything runs through libstx.so (hand-written CUDA behind the C ABI of include/stx.h).
 Importing this package fails if the native libraries are missing: there is no CPU path.
@@ -47,8 +48,12 @@ def sparse_mlp_forward(x, concat_weight, active_down_weight, down_buf, combined_
 
 from .layer import SparseLayer, SparseStack  # noqa: E402
 from .skip import FastLoRAProjection, SkipMLP, compute_binary_mask  # noqa: E402
+from .rope import RotaryPositions, rotary_frequencies  # noqa: E402
+from .kv_cache import KVCache, KVLayer  # noqa: E402
+from .draft import draft_masks, tree_attention, verify_draft  # noqa: E402
 
 __all__ = [
     "WeightCache", "sparse_mlp_forward", "approx_topk_threshold",
     "SparseLayer", "SparseStack", "FastLoRAProjection", "SkipMLP", "compute_binary_mask",
+    "RotaryPositions", "rotary_frequencies", "KVCache", "KVLayer", "draft_masks", "tree_attention", "verify_draft",
 ]

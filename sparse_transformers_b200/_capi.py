@@ -29,6 +29,30 @@ _pp = ctypes.POINTER(ctypes.c_void_p)
 _pi64 = ctypes.POINTER(ctypes.c_int64)
 _psz = ctypes.POINTER(ctypes.c_size_t)
 
+STORE_SAME, STORE_INT8, STORE_E4M3 = range(3)
+DRAFT_MAX = 64
+VERIFY_MAX_VOCAB = 400000
+
+
+class KV(ctypes.Structure):
+    """stx_kv"""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("seq_stride", _i64), ("head_stride", _i64), ("slot_stride", _i64),
+                ("scale_seq_stride", _i64), ("scale_head_stride", _i64), ("max_len", _i64),
+                ("n_seq", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("store", _i32), ("dtype", _i32)]
+
+
+class Heads(ctypes.Structure):
+    """stx_heads"""
+    _fields_ = [("data", _vp), ("seq_stride", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class Rotary(ctypes.Structure):
+    """stx_rotary"""
+    _fields_ = [("turns", _vp), ("rotary_dim", _i32), ("interleaved", _i32), ("factor", ctypes.c_double)]
+
+
+_pkv, _pheads, _prot = ctypes.POINTER(KV), ctypes.POINTER(Heads), ctypes.POINTER(Rotary)
+
 # name -> (restype, argtypes); mirrors include/stx.h one to one
 SIGNATURES = {
     "stx_last_error": (ctypes.c_char_p, []),
@@ -86,6 +110,14 @@ SIGNATURES = {
     "stx_add_rmsnorm": (_i32, [_vp, _vp, _vp, ctypes.c_float, _vp, _vp, _i64, _i32, _vp]),
     "stx_decode_finish": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
     "stx_norm_gemv": (_i32, [_vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "stx_rope": (_i32, [_pheads, _pheads, _i64, _i64, _i32, _i32, _vp, _i64, _prot, _i32, _i32, _vp]),
+    "stx_kv_append": (_i32, [_pkv, _pheads, _pheads, _i64, _vp, _vp, _prot, _vp, _i64, _pheads, _pheads, _i32, _vp]),
+    "stx_kv_read": (_i32, [_pkv, _vp, _i64, _vp, _vp, _vp]),
+    "stx_kv_keep": (_i32, [_pkv, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "stx_draft_masks": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp]),
+    "stx_tree_attention_workspace_bytes": (_i32, [_i64, _i32, _i32, _i32, _i32, _psz]),
+    "stx_tree_attention": (_i32, [_pkv, _pheads, _pheads, _i64, _i32, _f32, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "stx_verify_draft": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
 }
 
 

@@ -20,7 +20,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIBSTX = os.path.join(HERE, "libstx.so")
 LIBSHIM = os.path.join(HERE, "libstx_torch.so")
 
-CU_SOURCES = ["stx_api.cu", "stx_cache.cu", "stx_predictor.cu", "stx_select.cu", "stx_mlp.cu", "stx_mlp_tma.cu", "stx_mlp_batch.cu", "stx_mlp_row.cu", "stx_stack_b1.cu", "stx_stack_flow.cu", "stx_prefill.cu", "stx_peer.cu", "stx_attn.cu", "stx_layer.cu"]
+CU_SOURCES = ["stx_api.cu", "stx_cache.cu", "stx_predictor.cu", "stx_select.cu", "stx_mlp.cu", "stx_mlp_tma.cu", "stx_mlp_batch.cu", "stx_mlp_row.cu", "stx_stack_b1.cu", "stx_stack_flow.cu", "stx_prefill.cu", "stx_peer.cu", "stx_attn.cu", "stx_layer.cu", "stx_kv.cu", "stx_tree_attn.cu", "stx_draft.cu"]
+SHIM_SOURCES = ["torch_shim.cpp", "torch_shim_draft.cpp"]
 
 def _newer(target: str, sources: list[str]) -> bool:
     if not os.path.isfile(target):
@@ -58,8 +59,8 @@ def build_libstx(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_shim(force: bool = False, verbose: bool = False) -> str:
-    src = os.path.join(CSRC, "torch_shim.cpp")
-    if not force and _newer(LIBSHIM, [src, os.path.join(INCLUDE, "stx.h"), LIBSTX]):
+    srcs = [os.path.join(CSRC, f) for f in SHIM_SOURCES]
+    if not force and _newer(LIBSHIM, srcs + [os.path.join(INCLUDE, "stx.h"), LIBSTX]):
         return LIBSHIM
     import torch
     from torch.utils import cpp_extension as ce
@@ -69,7 +70,7 @@ def build_shim(force: bool = False, verbose: bool = False) -> str:
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [f"-I{p}" for p in incs]
-    cmd += [src, "-o", LIBSHIM, f"-L{HERE}", "-lstx", "-Wl,-rpath,$ORIGIN",
+    cmd += srcs + ["-o", LIBSHIM, f"-L{HERE}", "-lstx", "-Wl,-rpath,$ORIGIN",
             f"-L{torch_lib}", f"-Wl,-rpath,{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
             f"-L{os.path.join(cuda_home(), 'lib64')}", "-lcudart"]
     _run(cmd, verbose)

@@ -1,0 +1,135 @@
+// How stx_tree_attention's work is shared out (host and both kernels).
+//
+// A unit is (sequence, cache head, row tile): rows = tokens x query heads of the cache head, ROWS at most, token major.  Its
+// keys are cut into tiles of KT slots.  All tiles of all units stand in one line, and CTA c of G takes the tiles
+// [W c / G, W (c + 1) / G): every CTA has the same number of tiles (off by one at most) whatever the lengths, which only the
+// device knows.  A CTA's first and last unit may be shared with its neighbours; their partial sums (accumulator, maximum, sum
+// of exponentials) go to slots 2 c and 2 c + 1 of the workspace and a second launch adds them in CTA order, so that the result does not depend on
+// timing.  What lies between is finished by the CTA itself.
+#pragma once
+
+#include "stx_kv.cuh"
+
+namespace stx {
+
+constexpr int TREE_MAX_SEQ = 1024;
+
+struct TreeArgs {
+  const void* q;
+  void* out;
+  int64_t q_seq, q_tok, q_head, o_seq, o_tok, o_head;
+  const int64_t *length, *counts, *masks;
+  int64_t mask_stride;
+  int64_t max_len;
+  float scale_log2;  // scale * log2(e): soft-max in powers of two
+  int n_seq, n_tok, nkv, group, hd;
+  int tile_tok, row_tiles;  // tokens of a row tile, row tiles of a (sequence, cache head)
+  int min_tiles;            // fewest tiles that are worth a CTA of their own
+  int grid;                 // CTAs of the first launch
+  float* part;              // [2 grid][hd / 4][ROWS][4], then [2 grid][2][ROWS]
+};
+
+struct TreeSeq {
+  int len, cnt, keys;  // prefix, nodes, slots looked at
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
+  TreeSeq s;
+  s.len = static_cast<int>(min(static_cast<long long>(a.max_len), max(0ll, static_cast<long long>(a.length[b]))));
+  s.cnt = a.counts ? static_cast<int>(min(static_cast<long long>(a.n_tok), max(0ll, static_cast<long long>(a.counts[b])))) : a.n_tok;
+  s.keys = s.cnt > 0 ? s.len + min(s.cnt, static_cast<int>(a.max_len) - s.len) : 0;
+  return s;
+}
+// A sequence without keys still has a tile: its rows are written (as zeros) by somebody.
+__device__ __forceinline__ int tree_tiles(int keys, int kt) { return keys > 0 ? (keys + kt - 1) / kt : 1; }
+
+// pre[b] = tiles of a row tile of one cache head, summed over the sequences before b; pre[n_seq] the sum.  By warp 0; the
+// caller synchronises.
+__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int kt, long long* pre) {
+  if (threadIdx.x >= 32) return;
+  long long base = 0;
+  for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    const long long own = b < a.n_seq ? tree_tiles(tree_seq(a, b).keys, kt) : 0;
+    long long sum = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, sum, off);
+      if (static_cast<int>(threadIdx.x) >= off) sum += o;
+    }
+    if (b < a.n_seq) pre[b] = base + sum - own;
+    base += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (threadIdx.x == 0) pre[a.n_seq] = base;
+}
+
+struct TreeLine {
+  long long total;  // W
+  long long ctas;   // G
+  long long per;    // units of a sequence
+};
+__device__ __forceinline__ TreeLine tree_line(const TreeArgs& a, const long long* pre) {
+  TreeLine l;
+  l.per = static_cast<long long>(a.nkv) * a.row_tiles;
+  l.total = pre[a.n_seq] * l.per;
+  l.ctas = max(1ll, min(static_cast<long long>(a.grid), l.total / a.min_tiles));
+  return l;
+}
+__device__ __forceinline__ long long tree_begin(const TreeLine& l, long long c) { return l.total * c / l.ctas; }
+__device__ __forceinline__ long long tree_owner(const TreeLine& l, long long x) { return ((x + 1) * l.ctas - 1) / l.total; }
+
+// The unit at position x of the line, and the part of [x, end) that lies in it.
+struct TreeSeg {
+  int b, head, rt;
+  int t0, t1, nt;        // tiles of this segment, tiles of the unit
+  long long first;       // position of the unit's first tile
+};
+__device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, const TreeLine& l, const long long* pre, long long x, long long end) {
+  int lo = 0, hi = a.n_seq - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] * l.per <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  TreeSeg s;
+  s.b = lo;
+  s.nt = static_cast<int>(pre[lo + 1] - pre[lo]);
+  const long long in = x - pre[lo] * l.per;
+  const int u = static_cast<int>(in / s.nt);
+  s.t0 = static_cast<int>(in - static_cast<long long>(u) * s.nt);
+  s.t1 = static_cast<int>(min(static_cast<long long>(s.nt), s.t0 + end - x));
+  s.first = x - s.t0;
+  s.head = u / a.row_tiles;
+  s.rt = u - s.head * a.row_tiles;
+  return s;
+}
+
+// Bits of 32 slots from s0 on that a node sees: slots below len, nodes by `bits` (already cut to the nodes in use).
+__device__ __forceinline__ uint32_t tree_visible(int s0, int len, unsigned long long bits) {
+  const int rel = s0 - len;
+  if (rel >= 64) return 0u;
+  if (rel >= 0) return static_cast<uint32_t>(bits >> rel);
+  if (rel <= -32) return 0xffffffffu;
+  return static_cast<uint32_t>(bits << -rel) | ((1u << -rel) - 1u);
+}
+// Nodes that row token t sees (0 for a token that is not in use), without those behind the cache's end.
+__device__ __forceinline__ unsigned long long tree_bits(const TreeArgs& a, const TreeSeq& s, int b, int t) {
+  if (t >= s.cnt) return 0ull;
+  const unsigned long long m = a.masks ? static_cast<unsigned long long>(a.masks[b * a.mask_stride + t]) : ~0ull >> (63 - t);
+  const int nodes = s.keys - s.len;
+  return nodes <= 0 ? 0ull : m & (~0ull >> (64 - nodes));
+}
+
+__host__ __device__ constexpr size_t tree_part_floats(int grid, int rows, int hd) {
+  return static_cast<size_t>(2 * grid) * rows * (static_cast<size_t>((hd + 3) / 4) * 4 + 2);
+}
+__device__ __forceinline__ float* tree_part_o(const TreeArgs& a, int rows, long long slot) {
+  return a.part + static_cast<size_t>(slot) * rows * (((a.hd + 3) / 4) * 4);
+}
+__device__ __forceinline__ float* tree_part_ml(const TreeArgs& a, int rows, long long slot) {
+  return a.part + static_cast<size_t>(2 * a.grid) * rows * (((a.hd + 3) / 4) * 4) + static_cast<size_t>(slot) * 2 * rows;
+}
+
+// Adds the partial results of shared units; ROWS as in the first launch.
+int launch_tree_join(const TreeArgs& a, int rows, int kt, int dtype, cudaStream_t s);
+
+}  // namespace stx

@@ -1,0 +1,113 @@
+"""Rotary positions: half and interleaved layouts, part of the head, scaled for long contexts.
+
+The reference takes rotary embeddings from transformers (src/models/llama/modelling_llama_skip.py); here the angle of a pair is
+formed inside the kernel, in fp64, so there is no table and no largest position.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+_rope = torch.ops.sparse_mlp.rope.default
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[dict] = None) -> tuple[list[float], float]:
+    """(radians per position of each of the rotary_dim / 2 pairs, factor of the result).
+
+    Unscaled: theta^(-2 i / rotary_dim).  ``scaling`` has a ``rope_type`` and a ``factor``, and as transformers names them:
+      linear   every frequency / factor
+      ntk      theta * factor^(d / (d - 2)): the slowest pair is slowed by factor, the fastest left alone
+      llama3   pairs that turn less than low_freq_factor times within original_max_position_embeddings are slowed by factor,
+               those that turn more than high_freq_factor times are left alone, between them a linear blend
+      yarn     the same idea, blended linearly over the pair's index between the pairs that turn beta_fast (32) and beta_slow (1)
+               times; the result is multiplied by attention_factor (default 0.1 ln(factor) + 1)"""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be positive and even, not {rotary_dim}")
+    if not theta > 0:
+        raise ValueError(f"theta must be positive, not {theta}")
+    kind = "none" if scaling is None else scaling.get("rope_type", scaling.get("type", "none"))
+    if kind in ("none", "default"):
+        scaling, kind = {}, "none"
+    factor = float(scaling.get("factor", 1.0))
+    if not factor > 0:
+        raise ValueError(f"factor must be positive, not {factor}")
+    if kind == "ntk" and rotary_dim > 2:
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    w = [theta ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if kind in ("none", "ntk"):
+        return w, 1.0
+    if kind == "linear":
+        return [x / factor for x in w], 1.0
+    if kind not in ("llama3", "yarn"):
+        raise ValueError(f"unknown rope_type {kind!r} (linear, ntk, llama3, yarn)")
+    if "original_max_position_embeddings" not in scaling:
+        raise ValueError(f"rope_type {kind!r} needs original_max_position_embeddings")
+    orig = float(scaling["original_max_position_embeddings"])
+    if kind == "llama3":
+        lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not hi > lo:
+            raise ValueError("high_freq_factor must be above low_freq_factor")
+        keep = [min(1.0, max(0.0, (orig * x / (2 * math.pi) - lo) / (hi - lo))) for x in w]
+        return [x * (k + (1.0 - k) / factor) for x, k in zip(w, keep)], 1.0
+    index = lambda turns: rotary_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta))
+    lo = max(math.floor(index(float(scaling.get("beta_fast", 32.0)))), 0)
+    hi = min(math.ceil(index(float(scaling.get("beta_slow", 1.0)))), rotary_dim - 1)
+    slow = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(rotary_dim // 2)]
+    given = scaling.get("attention_factor")
+    return ([x * (1.0 - s + s / factor) for x, s in zip(w, slow)],
+            float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0))
+
+
+class _Rotate(torch.autograd.Function):
+    """The rotation is linear: its gradient is the transposed rotation."""
+
+    @staticmethod
+    def forward(ctx, x, positions, plan, inverse):
+        ctx.positions, ctx.plan, ctx.inverse = positions, plan, inverse
+        with torch.no_grad():
+            return _rope(x, positions, plan.turns, plan.interleaved, plan.factor, inverse, None)
+
+    @staticmethod
+    def backward(ctx, g):
+        g = g if g.stride(-1) == 1 else g.contiguous()
+        return _Rotate.apply(g, ctx.positions, ctx.plan, not ctx.inverse), None, None, None
+
+
+class RotaryPositions:
+    """The rotary plan of a model: which values of a head form pairs and how fast each pair turns.
+
+    head_dim: values of a head; rotary_dim: how many of the first ones are rotated (default all); layout: "half" (pairs
+    (i, i + rotary_dim / 2)) or "interleaved" (pairs (2 i, 2 i + 1)); theta, scaling: see rotary_frequencies."""
+
+    def __init__(self, head_dim: int, *, rotary_dim: Optional[int] = None, theta: float = 10000.0, layout: str = "half",
+                 scaling: Optional[dict] = None, device: torch.device | str = "cuda"):
+        self.head_dim = int(head_dim)
+        self.rotary_dim = self.head_dim if rotary_dim is None else int(rotary_dim)
+        if not 0 < self.rotary_dim <= self.head_dim:
+            raise ValueError(f"rotary_dim {rotary_dim} of a head of {head_dim}")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout must be 'half' or 'interleaved', not {layout!r}")
+        self.interleaved = layout == "interleaved"
+        self.frequencies, self.factor = rotary_frequencies(self.rotary_dim, theta, scaling)
+        self.turns = torch.tensor([w / (2 * math.pi) for w in self.frequencies], dtype=torch.float64, device=device)
+
+    def rotate(self, x: torch.Tensor, positions: torch.Tensor, *, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [n, heads, head_dim] or [n_seq, n_tokens, heads, head_dim] (any strides with contiguous heads), positions int64
+        x.shape[:-2] -> the rotated tensor (``out``, which may be x, or a new one).  ``inverse`` applies the transposed map:
+        turned back and multiplied by the same factor.  Differentiable in x without ``out``."""
+        if x.shape[-1] != self.head_dim:
+            raise RuntimeError(f"rope: heads of {x.shape[-1]} values, the plan has {self.head_dim}")
+        if x.requires_grad and torch.is_grad_enabled() and out is None:
+            return _Rotate.apply(x, positions, self, inverse)
+        return _rope(x, positions, self.turns, self.interleaved, self.factor, inverse, out)
+
+    def tables(self, max_len: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """cos and sin [max_len, head_dim] in fp32 for stx_attn_decode, which rotates whole heads in the half layout."""
+        if self.interleaved or self.rotary_dim != self.head_dim:
+            raise ValueError("tables serve the half layout over the whole head")
+        a = torch.arange(max_len, dtype=torch.float64, device=self.turns.device)[:, None] * self.turns
+        a = 2 * math.pi * (a - a.round())
+        a = torch.cat([a, a], dim=-1)
+        return (a.cos() * self.factor).float(), (a.sin() * self.factor).float()
