@@ -318,6 +318,7 @@ int stx_tree_attention(const stx_kv* cache, const stx_heads* q, const stx_heads*
   a.group = group;
   a.hd = cache->head_dim;
   a.part = static_cast<float*>(workspace);
+  if (tree_mma_wanted(cache)) return tree_mma(a, cache, s);
   const int rows = group * a.n_tok > 16 ? 64 : 16;  // 64 rows read a key four times less often, 16 leave fewer of them empty
   a.tile_tok = std::min(a.n_tok, rows / group);
   a.row_tiles = (a.n_tok + a.tile_tok - 1) / a.tile_tok;

@@ -132,4 +132,8 @@ __device__ __forceinline__ float* tree_part_ml(const TreeArgs& a, int rows, long
 // Adds the partial results of shared units; ROWS as in the first launch.
 int launch_tree_join(const TreeArgs& a, int rows, int kt, int dtype, cudaStream_t s);
 
+// The tensor-core kernel (stx_tree_attn_mma.cu): 16-bit models, caches that a tensor map can describe.
+bool tree_mma_wanted(const stx_kv* cache);
+int tree_mma(TreeArgs a, const stx_kv* cache, cudaStream_t s);
+
 }  // namespace stx
