@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) k_tree_attn_any(const TreeArgs 
                                                                const KvPtr<typename Held<T, STORE>::C> vc, int vec) {
   typedef typename Held<T, STORE>::C C;
   extern __shared__ __align__(16) float tg[];
-  __shared__ long long pre[TREE_MAX_SEQ + 1];
+  __shared__ int pre[TREE_MAX_SEQ + 1];
   __shared__ unsigned long long bits_s[ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hdp = (a.hd + 3) / 4 * 4, d4n = hdp / 4;
@@ -39,11 +39,10 @@ __global__ void __launch_bounds__(TG_THREADS, 1) k_tree_attn_any(const TreeArgs 
   tree_prefix(a, TG_KT, pre);
   __syncthreads();
   const TreeLine line = tree_line(a, pre);
-  const long long cta = blockIdx.x;
+  const int cta = blockIdx.x;
   if (cta >= line.ctas) return;
-  const long long end = tree_begin(line, cta + 1);
-  const long long begin = tree_begin(line, cta);
-  for (long long x = begin; x < end;) {
+  const int end = tree_begin(line, cta + 1), begin = tree_begin(line, cta);
+  for (int x = begin; x < end;) {
     const TreeSeg sg = tree_seg(a, line, pre, x, end);
     const TreeSeq sq = tree_seq(a, sg.b);
     const int tok0 = sg.rt * a.tile_tok, rows = min(a.tile_tok, a.n_tok - tok0) * a.group;
@@ -151,7 +150,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) k_tree_attn_any(const TreeArgs 
       }
     }
     const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
-    const long long slot = 2 * cta + (x == begin ? 0 : 1);
+    const int slot = 2 * cta + (x == begin ? 0 : 1);
     float* po = tree_part_o(a, ROWS, slot);
 #pragma unroll
     for (int k = 0; k < TASKS; ++k) {
@@ -183,41 +182,66 @@ __global__ void __launch_bounds__(TG_THREADS, 1) k_tree_attn_any(const TreeArgs 
   }
 }
 
-// Block (c, y): the unit that begins in CTA c's tiles and ends behind them, four groups of four values of its rows.
-//   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the CTAs i = c, c + 1, .. that have a part of it, in that order
+constexpr int TJ_THREADS = 256;
+// Blocks (c, y): the unit that begins in CTA c's tiles and ends behind them; a thread has four values of a row.
+//   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the CTAs i = c, c + 1, .. that have a part of it, in that order,
+// eight parts' loads in flight at a time.  Lengths and counts are inputs of the launch before, which has waited for whoever wrote them:
+// the unit is found while that launch still runs.
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(4 * ROWS) k_tree_join(const TreeArgs a, int kt) {
-  __shared__ long long pre[TREE_MAX_SEQ + 1];
-  pdl_wait();
-  pdl_launch_dependents();
+__global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const TreeArgs a, int kt) {
+  __shared__ int pre[TREE_MAX_SEQ + 1];
   tree_prefix(a, kt, pre);
   __syncthreads();
   const TreeLine line = tree_line(a, pre);
-  const long long cta = blockIdx.x;
-  if (cta + 1 >= line.ctas) return;
-  const long long end = tree_begin(line, cta + 1), begin = tree_begin(line, cta);
+  const int cta = blockIdx.x;
+  bool mine = cta + 1 < line.ctas;
+  const int end = mine ? tree_begin(line, cta + 1) : 1, begin = mine ? tree_begin(line, cta) : 0;
   const TreeSeg sg = tree_seg(a, line, pre, end - 1, end);
-  if (sg.first < begin || sg.first + sg.nt <= end) return;
-  const int parts = static_cast<int>(tree_owner(line, sg.first + sg.nt - 1) - cta) + 1;
-  const int row = threadIdx.x % ROWS, d4 = blockIdx.y * 4 + threadIdx.x / ROWS;
+  mine = mine && sg.first >= begin && sg.first + sg.nt > end;
+  const int rows = min(a.tile_tok, a.n_tok - sg.rt * a.tile_tok) * a.group;
+  const int item = blockIdx.y * TJ_THREADS + threadIdx.x, d4 = item / rows, row = item - d4 * rows;
   const int tok = sg.rt * a.tile_tok + row / a.group;
-  if (row >= a.tile_tok * a.group || tok >= a.n_tok || 4 * d4 >= a.hd) return;
+  mine = mine && 4 * d4 < a.hd;
+  const int parts = mine ? tree_owner(line, sg.first + sg.nt - 1) - cta + 1 : 0;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!mine) return;
   // CTA c ends with this unit: its first slot when the unit is all it has, else its second; those behind begin with it
-  auto slot_of = [&](int i) { return 2 * (cta + i) + (i == 0 && sg.first != begin ? 1 : 0); };
-  float M = -INFINITY;
-  for (int i = 0; i < parts; ++i) M = fmaxf(M, __ldcg(tree_part_ml(a, ROWS, slot_of(i)) + row));
-  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float* ml = tree_part_ml(a, ROWS, slot_of(i));
-    const float m = __ldcg(ml + row), li = __ldcg(ml + ROWS + row);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(tree_part_o(a, ROWS, slot_of(i)) + (static_cast<size_t>(d4) * ROWS + row) * 4));
-    const float f = m == -INFINITY && li == 0.f ? 0.f : exp2f(m - M);  // a part that has seen nothing
-    l = fmaf(li, f, l);
-    o[0] = fmaf(v.x, f, o[0]);
-    o[1] = fmaf(v.y, f, o[1]);
-    o[2] = fmaf(v.z, f, o[2]);
-    o[3] = fmaf(v.w, f, o[3]);
+  const int slot0 = 2 * cta + (sg.first == begin ? 0 : 1);
+  float M = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < parts; i0 += 8) {
+    float m[8], li[8];
+    float4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int slot = i0 + k == 0 ? slot0 : 2 * (cta + i0 + k);
+      m[k] = -INFINITY;
+      li[k] = 0.f;
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + k < parts) {
+        const float* ml = tree_part_ml(a, ROWS, slot);
+        m[k] = __ldcg(ml + row);
+        li[k] = __ldcg(ml + ROWS + row);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(tree_part_o(a, ROWS, slot) + (static_cast<size_t>(d4) * ROWS + row) * 4));
+      }
+    }
+    float up = M;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) up = fmaxf(up, m[k]);
+    const float f0 = M == up ? 1.f : exp2f(M - up);
+    M = up;
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = m[k] == -INFINITY && li[k] == 0.f ? 0.f : exp2f(m[k] - M);  // a part that has seen nothing
+      l = fmaf(li[k], f, l);
+      o[0] = fmaf(v[k].x, f, o[0]);
+      o[1] = fmaf(v[k].y, f, o[1]);
+      o[2] = fmaf(v[k].z, f, o[2]);
+      o[3] = fmaf(v[k].w, f, o[3]);
+    }
   }
   T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + tok * a.o_tok + (sg.head * a.group + row % a.group) * a.o_head + 4 * d4;
 #pragma unroll
@@ -226,12 +250,13 @@ __global__ void __launch_bounds__(4 * ROWS) k_tree_join(const TreeArgs a, int kt
 }
 
 int launch_tree_join(const TreeArgs& a, int rows, int kt, int dtype, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.grid), static_cast<unsigned>((a.hd + 15) / 16));
+  const int items = a.tile_tok * a.group * ((a.hd + 3) / 4);
+  const dim3 grid(static_cast<unsigned>(a.grid), static_cast<unsigned>((items + TJ_THREADS - 1) / TJ_THREADS));
   return by_dtype(dtype, [&](auto tag) -> int {
     typedef decltype(tag) T;
-    if (rows == 16) STX_CUDA(launch_pdl(k_tree_join<T, 16>, grid, dim3(64), 0, s, a, kt));
-    else if (rows == 64) STX_CUDA(launch_pdl(k_tree_join<T, 64>, grid, dim3(256), 0, s, a, kt));
-    else STX_CUDA(launch_pdl(k_tree_join<T, 128>, grid, dim3(512), 0, s, a, kt));
+    if (rows == 16) STX_CUDA(launch_pdl(k_tree_join<T, 16>, grid, dim3(TJ_THREADS), 0, s, a, kt));
+    else if (rows == 64) STX_CUDA(launch_pdl(k_tree_join<T, 64>, grid, dim3(TJ_THREADS), 0, s, a, kt));
+    else STX_CUDA(launch_pdl(k_tree_join<T, 128>, grid, dim3(TJ_THREADS), 0, s, a, kt));
     return STX_OK;
   });
 }
@@ -318,6 +343,9 @@ int stx_tree_attention(const stx_kv* cache, const stx_heads* q, const stx_heads*
   a.group = group;
   a.hd = cache->head_dim;
   a.part = static_cast<float*>(workspace);
+  // the line of tiles is counted in 32 bits; a cache that fits a device is far below
+  STX_CHECK_ARG(static_cast<double>(cache->n_seq) * cache->n_kv_heads * n_tokens * (static_cast<double>(cache->max_len) / 64 + 1) < 2147483648.0,
+                "stx_tree_attention: n_seq * n_kv_heads * n_tokens * max_len is too large");
   if (tree_mma_wanted(cache)) return tree_mma(a, cache, s);
   const int rows = group * a.n_tok > 16 ? 64 : 16;  // 64 rows read a key four times less often, 16 leave fewer of them empty
   a.tile_tok = std::min(a.n_tok, rows / group);

@@ -1,9 +1,8 @@
 // How stx_tree_attention's work is shared out (host and both kernels).
 //
 // A unit is (sequence, cache head, row tile): rows = tokens x query heads of the cache head, ROWS at most, token major.  Its
-// keys are cut into tiles of KT slots.  All tiles of all units stand in one line, and CTA c of G takes the tiles
-// [W c / G, W (c + 1) / G): every CTA has the same number of tiles (off by one at most) whatever the lengths, which only the
-// device knows.  A CTA's first and last unit may be shared with its neighbours; their partial sums (accumulator, maximum, sum
+// keys are cut into tiles of KT slots.  All tiles of all units stand in one line, and each of G CTAs takes an equal stretch of it:
+// the same number of tiles (off by one at most) whatever the lengths, which only the device knows.  A CTA's first and last unit may be shared with its neighbours; their partial sums (accumulator, maximum, sum
 // of exponentials) go to slots 2 c and 2 c + 1 of the workspace and a second launch adds them in CTA order, so that the result does not depend on
 // timing.  What lies between is finished by the CTA itself.
 #pragma once
@@ -43,17 +42,17 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
 __device__ __forceinline__ int tree_tiles(int keys, int kt) { return keys > 0 ? (keys + kt - 1) / kt : 1; }
 
 // pre[b] = tiles of a row tile of one cache head, summed over the sequences before b; pre[n_seq] the sum.  By warp 0; the
-// caller synchronises.
-__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int kt, long long* pre) {
+// caller synchronises.  The host has made sure that the whole line has less than 2^31 tiles.
+__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int kt, int* pre) {
   if (threadIdx.x >= 32) return;
-  long long base = 0;
+  int base = 0;
   for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    const long long own = b < a.n_seq ? tree_tiles(tree_seq(a, b).keys, kt) : 0;
-    long long sum = own;
+    const int own = b < a.n_seq ? tree_tiles(tree_seq(a, b).keys, kt) : 0;
+    int sum = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, sum, off);
+      const int o = __shfl_up_sync(0xffffffffu, sum, off);
       if (static_cast<int>(threadIdx.x) >= off) sum += o;
     }
     if (b < a.n_seq) pre[b] = base + sum - own;
@@ -63,27 +62,32 @@ __device__ __forceinline__ void tree_prefix(const TreeArgs& a, int kt, long long
 }
 
 struct TreeLine {
-  long long total;  // W
-  long long ctas;   // G
-  long long per;    // units of a sequence
+  int total, ctas;  // W, G
+  int each, more;   // W / G; the first W mod G CTAs have one tile more
+  int per;          // units of a sequence
 };
-__device__ __forceinline__ TreeLine tree_line(const TreeArgs& a, const long long* pre) {
+__device__ __forceinline__ TreeLine tree_line(const TreeArgs& a, const int* pre) {
   TreeLine l;
-  l.per = static_cast<long long>(a.nkv) * a.row_tiles;
+  l.per = a.nkv * a.row_tiles;
   l.total = pre[a.n_seq] * l.per;
-  l.ctas = max(1ll, min(static_cast<long long>(a.grid), l.total / a.min_tiles));
+  l.ctas = max(1, min(a.grid, l.total / a.min_tiles));
+  l.each = l.total / l.ctas;
+  l.more = l.total - l.each * l.ctas;
   return l;
 }
-__device__ __forceinline__ long long tree_begin(const TreeLine& l, long long c) { return l.total * c / l.ctas; }
-__device__ __forceinline__ long long tree_owner(const TreeLine& l, long long x) { return ((x + 1) * l.ctas - 1) / l.total; }
+__device__ __forceinline__ int tree_begin(const TreeLine& l, int c) { return l.each * c + min(c, l.more); }
+__device__ __forceinline__ int tree_owner(const TreeLine& l, int x) {
+  const int cut = l.more * (l.each + 1);
+  return x < cut ? x / (l.each + 1) : l.more + (x - cut) / l.each;
+}
 
 // The unit at position x of the line, and the part of [x, end) that lies in it.
 struct TreeSeg {
   int b, head, rt;
-  int t0, t1, nt;        // tiles of this segment, tiles of the unit
-  long long first;       // position of the unit's first tile
+  int t0, t1, nt;  // tiles of this segment, tiles of the unit
+  int first;       // position of the unit's first tile
 };
-__device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, const TreeLine& l, const long long* pre, long long x, long long end) {
+__device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, const TreeLine& l, const int* pre, int x, int end) {
   int lo = 0, hi = a.n_seq - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -92,11 +96,10 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, const TreeLine& l
   }
   TreeSeg s;
   s.b = lo;
-  s.nt = static_cast<int>(pre[lo + 1] - pre[lo]);
-  const long long in = x - pre[lo] * l.per;
-  const int u = static_cast<int>(in / s.nt);
-  s.t0 = static_cast<int>(in - static_cast<long long>(u) * s.nt);
-  s.t1 = static_cast<int>(min(static_cast<long long>(s.nt), s.t0 + end - x));
+  s.nt = pre[lo + 1] - pre[lo];
+  const int in = x - pre[lo] * l.per, u = in / s.nt;
+  s.t0 = in - u * s.nt;
+  s.t1 = min(s.nt, s.t0 + end - x);
   s.first = x - s.t0;
   s.head = u / a.row_tiles;
   s.rt = u - s.head * a.row_tiles;
@@ -122,10 +125,10 @@ __device__ __forceinline__ unsigned long long tree_bits(const TreeArgs& a, const
 __host__ __device__ constexpr size_t tree_part_floats(int grid, int rows, int hd) {
   return static_cast<size_t>(2 * grid) * rows * (static_cast<size_t>((hd + 3) / 4) * 4 + 2);
 }
-__device__ __forceinline__ float* tree_part_o(const TreeArgs& a, int rows, long long slot) {
+__device__ __forceinline__ float* tree_part_o(const TreeArgs& a, int rows, int slot) {
   return a.part + static_cast<size_t>(slot) * rows * (((a.hd + 3) / 4) * 4);
 }
-__device__ __forceinline__ float* tree_part_ml(const TreeArgs& a, int rows, long long slot) {
+__device__ __forceinline__ float* tree_part_ml(const TreeArgs& a, int rows, int slot) {
   return a.part + static_cast<size_t>(2 * a.grid) * rows * (((a.hd + 3) / 4) * 4) + static_cast<size_t>(slot) * 2 * rows;
 }
 

@@ -32,32 +32,35 @@ namespace stx {
 
 constexpr int TM_ROWS = 128;
 constexpr float TM_SLACK = 8.f;  // in powers of two
-constexpr uint32_t TM_WAIT_LIMIT = 1u << 21;
+constexpr uint32_t TM_WAIT_LIMIT = 1u << 17;  // polls of up to 4 us: half a second
 
 template <int STORE, int HD> struct TmShape {
   static constexpr bool CODED = STORE != STX_STORE_SAME;
-  static constexpr int KT = HD == 256 ? 64 : 128;   // slots of a tile
+  static constexpr int KT = 64;                     // slots of a tile
   static constexpr int NS = HD == 256 ? 1 : 2;      // streams: two O of 256 columns do not fit next to S
+  static constexpr int NB = 2 * NS;                 // S buffers, two for each stream
   static constexpr int BOXES = HD / 64;             // 128-byte wide parts of an operand row
   static constexpr uint32_t BOX = KT * 128;         // bytes of such a part of a K or V tile
   static constexpr uint32_t TILE = BOXES * BOX;
   static constexpr uint32_t QBOX = TM_ROWS * 128, Q = BOXES * QBOX;
-  // Tiles in shared memory (16-bit): what an SM has to have on its way is 45 KB (0.3 KB/ns of HBM x 148 SMs at 1 us); the rest of 227 KB
-  // is Q, the codes and what belongs to the sequences.
-  static constexpr int DK = HD == 64 ? 4 : CODED ? 2 : HD == 128 ? 3 : 2;
-  static constexpr int DV = HD == 64 ? 4 : CODED && HD == 256 ? 1 : 2;
-  static constexpr int RAW = CODED ? (HD == 64 ? 6 : 3) : 0;  // tiles of codes, K and V in turn
+  // Tiles in shared memory (16-bit).  K runs ahead of V by the S that are formed in advance.  What an SM has to have on its way is 45 KB
+  // (0.3 KB/ns of HBM x 148 SMs at 1 us).
+  static constexpr int DK = HD == 64 ? (CODED ? 6 : 8) : HD == 128 ? (CODED ? 4 : 6) : 2;
+  static constexpr int DV = HD == 64 ? (CODED ? 4 : 6) : HD == 128 ? (CODED ? 3 : 5) : CODED ? 1 : 2;
+  static constexpr int RAW = CODED ? (HD == 64 ? 12 : HD == 128 ? 8 : 3) : 0;  // tiles of codes, K and V in turn
   static constexpr uint32_t RAW_TILE = KT * HD;
-  // Tiles whose scales are kept: those of tile n are overwritten with K of tile n + SCALES, which waits for S of tile n + SCALES - DK,
-  // which waited for the soft-max of tile n + SCALES - DK - NS.
-  static constexpr int SCALES = DK + NS;
-  static constexpr int WARPS = 4 * NS + 2 + (CODED ? 4 : 0);
+  // Tiles whose scales are kept: those of tile n are overwritten with K of tile n + SCALES, which waits for S of tile n + SCALES - DK = n + NB,
+  // the next S in the buffer of tile n, and so for the P of tile n.
+  static constexpr int SCALES = DK + NB;
+  static constexpr int ISSUERS = NS;                // warps that issue products, one for each stream
+  static constexpr int WARPS = 4 * NS + 1 + ISSUERS + (CODED ? 4 : 0);
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr uint32_t O_COL = 256, S_COLS = KT;
+  static constexpr uint32_t O_COL = 256;
   static constexpr uint32_t SMEM_TILES = Q + DK * TILE + DV * TILE + RAW * RAW_TILE;
   static constexpr uint32_t SMEM_SCALES = CODED ? SCALES * 3 * KT * 4 : 0;
-  static constexpr uint32_t BARS = 2 * DK + 2 * DV + 6 + 2 + 2 * RAW + SCALES;
+  static constexpr uint32_t BARS = 2 * DK + 2 * DV + 2 * NB + 2 * NS + 1 + NS + 2 * RAW + (CODED ? SCALES : 0);
   static constexpr uint32_t SMEM = 1024 + SMEM_TILES + SMEM_SCALES + 2 * 2 * TM_ROWS * 4 + BARS * 8 + 64;
+  static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1) + 64 <= 227 * 1024, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
@@ -71,6 +74,13 @@ __device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile
 }
 __device__ __forceinline__ void tm_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// One lane of a converged warp.  The roles that issue products and copies run as whole warps and only the issuing is left to this lane: in code
+// that a branch on the lane number has split off, descriptors cannot be taken for uniform, and each product cost twice its time.
+__device__ __forceinline__ bool tm_elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 __device__ __forceinline__ void tm_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -104,35 +114,42 @@ __device__ __forceinline__ void tm_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
       : "memory");
 }
-// 32 columns of the warp's 32 lanes; the values are there after tm_ld_wait().
-__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// Columns of the warp's 32 lanes.  The wait is part of the statement: between the two the compiler could move registers that are not
+// there yet (it does where it has to spill).
+__device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
       "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -154,6 +171,27 @@ template <typename T>
 __device__ __forceinline__ uint32_t tm_not_finite(uint32_t w) {
   constexpr uint32_t E = DT<T>::id == STX_F16 ? 0x7c00u : 0x7f80u;
   return ((w & E) == E ? 0x0000ffffu : 0u) | ((w >> 16 & E) == E ? 0xffff0000u : 0u);
+}
+
+// Eight 16-bit values, in one load where they are aligned.
+template <typename T>
+__device__ __forceinline__ uint4 tm_load8(const T* p, int vec) {
+  if (vec) return ld_cached16(p);
+  const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+  return make_uint4(u[0] | static_cast<uint32_t>(u[1]) << 16, u[2] | static_cast<uint32_t>(u[3]) << 16, u[4] | static_cast<uint32_t>(u[5]) << 16,
+                    u[6] | static_cast<uint32_t>(u[7]) << 16);
+}
+
+template <typename T>
+__device__ __forceinline__ void tm_store8(T* p, int vec, const uint4& v) {
+  if (vec) {
+    st16(p, v);
+    return;
+  }
+  unsigned short* u = reinterpret_cast<unsigned short*>(p);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)));
 }
 
 // Two 16-bit operands from two codes.  int8: the byte is put under the exponent of a number whose last place is 1, and that number
@@ -188,13 +226,13 @@ __device__ __forceinline__ bool tm_code_nan(uint32_t w) { return (((w & 0x7f7f7f
 
 // The tiles of a CTA, one after the other.
 struct TmWalk {
-  long long x, end;
+  int x, end;
   TreeSeg sg;
   TreeSeq sq;
   int t;
   bool begun;
 };
-__device__ __forceinline__ bool tm_next_segment(const TreeArgs& a, const TreeLine& l, const long long* pre, TmWalk& w) {
+__device__ __forceinline__ bool tm_next_segment(const TreeArgs& a, const TreeLine& l, const int* pre, TmWalk& w) {
   if (w.begun) w.x += w.sg.t1 - w.sg.t0;
   w.begun = true;
   if (w.x >= w.end) return false;
@@ -219,14 +257,71 @@ __device__ __forceinline__ void tm_load(void* dst, const CUtensorMap* m, int ord
       : "memory");
 }
 
+// The row's x of a tile from its S (16-bit caches: S itself), what it does not see as -infinity, and the largest of them.  TAIL: the tile has
+// slots that the row may not see; `cut` is 0 for rows that are not in use.  The two forms are apart so that the common one has no masks in it.
+template <int STORE, bool TAIL>
+__device__ __forceinline__ float tm_row_max(uint32_t (&r)[64], const float* sc, int s0, int len, unsigned long long bits, uint32_t cut) {
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  uint32_t v[2] = {~0u, ~0u};
+  if (TAIL) {
+    v[0] = tree_visible(s0, len, bits) & cut;
+    v[1] = tree_visible(s0 + 32, len, bits) & cut;
+  }
+#pragma unroll
+  for (int j = 0; j < 64; j += 4) {
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(r[j + e]);
+    if constexpr (STORE != STX_STORE_SAME) {
+      const float4 kk = *reinterpret_cast<const float4*>(sc + j), lv = *reinterpret_cast<const float4*>(sc + 64 + j);
+      x[0] = fmaf(x[0], kk.x, lv.x), x[1] = fmaf(x[1], kk.y, lv.y), x[2] = fmaf(x[2], kk.z, lv.z), x[3] = fmaf(x[3], kk.w, lv.w);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (TAIL) x[e] = (v[j / 32] >> ((j + e) & 31)) & 1u ? x[e] : -INFINITY;
+      mx[e] = fmaxf(mx[e], x[e]);
+      r[j + e] = __float_as_uint(x[e]);
+    }
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// P = 2^(x - base), packed in pairs, to the columns from p_addr on; returns the sum of the row's weights.
+template <typename T, int STORE, bool TAIL>
+__device__ __forceinline__ float tm_row_weights(const uint32_t (&r)[64], uint32_t p_addr, const float* sc, float c, float base) {
+  float l[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t p16[16];
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      float p[4], iv[4] = {1.f, 1.f, 1.f, 1.f};
+      if constexpr (STORE != STX_STORE_SAME) {
+        const float4 ii = *reinterpret_cast<const float4*>(sc + 128 + 32 * h + j);
+        iv[0] = ii.x, iv[1] = ii.y, iv[2] = ii.z, iv[3] = ii.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(r[32 * h + j + e]);
+        p[e] = tm_exp2(STORE != STX_STORE_SAME ? x - base : fmaf(x, c, -base));
+        if (TAIL && x == -INFINITY) p[e] = iv[e] = 0.f;  // not seen: c may be 0, 1 / v_scale infinite or NaN
+        l[e] = STORE != STX_STORE_SAME ? fmaf(p[e], iv[e], l[e]) : l[e] + p[e];
+      }
+      p16[j / 2] = tm_pack<T>(p[0], p[1]);
+      p16[j / 2 + 1] = tm_pack<T>(p[2], p[3]);
+    }
+    tm_st16(p_addr + 16 * h, p16);
+  }
+  return (l[0] + l[1]) + (l[2] + l[3]);
+}
+
 template <typename T, int STORE, int HD>
 __global__ void __launch_bounds__(TmShape<STORE, HD>::THREADS, 1)
 k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvPtr<typename Held<T, STORE>::C> kc,
                 const KvPtr<typename Held<T, STORE>::C> vc, int vec) {
   typedef TmShape<STORE, HD> Z;
-  constexpr int KT = Z::KT, NS = Z::NS, DK = Z::DK, DV = Z::DV;
+  constexpr int KT = Z::KT, NS = Z::NS, NB = Z::NB, DK = Z::DK, DV = Z::DV;
   extern __shared__ unsigned char tm_raw[];
-  __shared__ long long pre[TREE_MAX_SEQ + 1];
+  __shared__ int pre[TREE_MAX_SEQ + 1];
   __shared__ unsigned long long bad_s;  // nodes of the segment with a value that is not finite
   __shared__ uint32_t tmem_s;
   __shared__ int dead_s;
@@ -239,7 +334,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   float* ml_s = sc_s + Z::SMEM_SCALES / 4;                               // [2][2][TM_ROWS]
   uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + 2 * 2 * TM_ROWS);
   uint64_t *k_full = bars, *k_empty = k_full + DK, *v_full = k_empty + DK, *v_empty = v_full + DV, *s_full = v_empty + DV;
-  uint64_t *p_full = s_full + 2, *o_full = p_full + 2, *q_full = o_full + 2, *drain = q_full + 1, *raw_full = drain + 1;
+  uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + 1, *raw_full = drain + NS;
   uint64_t *raw_empty = raw_full + Z::RAW, *sc_full = raw_empty + Z::RAW;
   volatile int* dead = &dead_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -253,18 +348,22 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       mbar_init(&v_full[i], Z::CODED ? 4 : 1);
       mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NB; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
+      mbar_init(&drain[i], 1);
     }
     mbar_init(q_full, 4 * NS);
-    mbar_init(drain, 1);
     for (int i = 0; i < Z::RAW; ++i) {
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_empty[i], 4);
     }
-    for (int i = 0; i < Z::SCALES; ++i) mbar_init(&sc_full[i], 4);
+    if (Z::CODED)
+      for (int i = 0; i < Z::SCALES; ++i) mbar_init(&sc_full[i], 4);
     dead_s = 0;
     bad_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -274,7 +373,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   tree_prefix(a, KT, pre);
   __syncthreads();
   const TreeLine line = tree_line(a, pre);
-  const long long cta = blockIdx.x;
+  const int cta = blockIdx.x;
   if (cta >= line.ctas) return;
   if (warp == 4 * NS + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_s)) : "memory");
@@ -284,7 +383,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   __syncthreads();
   tm_fence_after();
   const uint32_t tmem = tmem_s;
-  const long long begin = tree_begin(line, cta);
+  const int begin = tree_begin(line, cta);
   TmWalk w;
   w.x = begin;
   w.end = tree_begin(line, cta + 1);
@@ -294,9 +393,10 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     // ------------------------------------------------------------------ softmax: a thread has a row
     const int st = warp >> 2, lg = warp & 3, row = lg * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(lg * 32) << 16);
-    const uint32_t s_addr = lane_base + st * Z::S_COLS, o_addr = lane_base + Z::O_COL + st * HD;
+    const uint32_t s_base = lane_base + st * 2 * KT, o_addr = lane_base + Z::O_COL + st * HD;
     const float c = fabsf(a.scale_log2);
-    uint32_t n_s = 0, n_o = 0;  // tiles and segments of this stream so far
+    uint32_t uses[2] = {0, 0};  // of the stream's two S buffers
+    uint32_t n_o = 0;           // segments in which the stream had a tile
     uint32_t tiles = 0;         // tiles of the CTA before this segment
     while (tm_next_segment(a, line, pre, w)) {
       const TreeSeg& sg = w.sg;
@@ -311,20 +411,21 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       {
         const T* src = static_cast<const T*>(a.q) + sg.b * a.q_seq + tok * a.q_tok + head * a.q_head;
         const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale goes with Q
-        for (int ch = st; ch < HD / 8; ch += NS) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (used && ch * 8 < a.hd) {  // hd is a multiple of 8
-            if (vec) {
-              v = ld_cached16(src + ch * 8);
-            } else {
-              T e[8];
+        constexpr int MINE = HD / 8 / NS, BATCH = MINE < 8 ? MINE : 8;  // 16-byte pieces of a row, requested together
+#pragma unroll 1
+        for (int c0 = 0; c0 < MINE; c0 += BATCH) {
+          uint4 v[BATCH];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) e[i] = src[ch * 8 + i];
-              v = *reinterpret_cast<const uint4*>(e);
-            }
-            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+          for (int i = 0; i < BATCH; ++i) {
+            const int ch = (c0 + i) * NS + st;
+            v[i] = used && ch * 8 < a.hd ? tm_load8(src + ch * 8, vec) : make_uint4(0, 0, 0, 0);  // hd is a multiple of 8
           }
-          *reinterpret_cast<uint4*>(q_t + (ch >> 3) * Z::QBOX + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int ch = (c0 + i) * NS + st;
+            const uint4 f = make_uint4(v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
+            *reinterpret_cast<uint4*>(q_t + (ch >> 3) * Z::QBOX + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = f;
+          }
         }
         tm_fence_async();
         __syncwarp();
@@ -333,11 +434,13 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       float m = -INFINITY, l = 0.f;
       const int nt = sg.t1 - sg.t0;
       for (int i = st; i < nt; i += NS) {
-        const int s0 = (sg.t0 + i) * KT;
+        const int s0 = (sg.t0 + i) * KT, buf = (i / NS) & 1;
         const bool tail = s0 + KT > sq.len;
         const uint32_t n = tiles + i;
+        const uint32_t s_addr = s_base + buf * KT;
         const float* sc = sc_s + (Z::CODED ? (n % Z::SCALES) * 3 * KT : 0);
-        bool ok = tm_wait(&s_full[st], n_s & 1, dead);
+        const uint32_t use = buf ? uses[1]++ : uses[0]++;
+        bool ok = tm_wait(&s_full[2 * st + buf], use & 1, dead);
         if (Z::CODED) ok = tm_wait(&sc_full[n % Z::SCALES], (n / Z::SCALES) & 1, dead) && ok;
         if (tail) {
           // slots behind the keys become zeros, and what is not finite in a node's value: 0 * NaN must not reach a row that
@@ -367,116 +470,45 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           }
         }
         ok = __all_sync(0xffffffffu, ok);
-        ++n_s;
         if (ok && warp_used) {
           tm_fence_after();
-          // ---- the row's largest x of this tile
-          float mx = -INFINITY;
-#pragma unroll
-          for (int c0 = 0; c0 < KT; c0 += 64) {
-            uint32_t r0[32], r1[32];
-            tm_ld32(s_addr + c0, r0);
-            tm_ld32(s_addr + c0 + 32, r1);
-            tm_ld_wait();
-            const uint32_t v0 = !tail ? 0xffffffffu : used ? tree_visible(s0 + c0, sq.len, bits) : 0u;
-            const uint32_t v1 = !tail ? 0xffffffffu : used ? tree_visible(s0 + c0 + 32, sq.len, bits) : 0u;
-            if constexpr (Z::CODED) {
-#pragma unroll
-              for (int j = 0; j < 64; j += 4) {
-                const float4 kk = *reinterpret_cast<const float4*>(sc + c0 + j), lv = *reinterpret_cast<const float4*>(sc + KT + c0 + j);
-                const float kx[4] = {kk.x, kk.y, kk.z, kk.w}, lx[4] = {lv.x, lv.y, lv.z, lv.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int jj = j + e;
-                  const float s = __uint_as_float(jj < 32 ? r0[jj & 31] : r1[jj & 31]);
-                  const float x = fmaf(s, kx[e], lx[e]);
-                  if (!tail || (((jj < 32 ? v0 : v1) >> (jj & 31)) & 1u)) mx = fmaxf(mx, x);
-                }
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                if (!tail || ((v0 >> j) & 1u)) mx = fmaxf(mx, __uint_as_float(r0[j]));
-                if (!tail || ((v1 >> j) & 1u)) mx = fmaxf(mx, __uint_as_float(r1[j]));
-              }
-            }
-          }
+          uint32_t r[64];
+          tm_ld64(s_addr, r);
+          const uint32_t cut = used ? 0xffffffffu : 0u;
+          float mx = tail ? tm_row_max<STORE, true>(r, sc, s0, sq.len, bits, cut) : tm_row_max<STORE, false>(r, sc, s0, sq.len, bits, cut);
           if (!Z::CODED && mx != -INFINITY) mx *= c;
           if (__any_sync(0xffffffffu, mx > m + TM_SLACK)) {
             const float up = mx > m + TM_SLACK ? mx : m;
             const float f = up == m ? 1.f : exp2f(m - up);
             m = up;
             l *= f;
-            if (i >= NS) {  // O holds something; this stream's products have completed
+            if (i >= NS) {  // O holds something: the stream's last product has to be in it
+              // Phase by parity: the one before it is over since S of this tile was formed, the one behind it waits for this tile's P.
+              const uint32_t done = uses[0] + uses[1] - 2;
+              ok = __all_sync(0xffffffffu, tm_wait(&pv_done[st], done & 1, dead));
+              tm_fence_after();
 #pragma unroll 1
-              for (int c0 = 0; c0 < HD; c0 += 32) {
-                uint32_t r[32];
-                tm_ld32(o_addr + c0, r);
-                tm_ld_wait();
+              for (int c0 = 0; c0 < HD; c0 += 16) {
+                uint32_t o[16];
+                tm_ld16(o_addr + c0, o);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
-                tm_st32(o_addr + c0, r);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                tm_st16(o_addr + c0, o);
               }
             }
           }
-          // ---- P and its sum
           const float base = m == -INFINITY ? 0.f : m;
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int c0 = 0; c0 < KT; c0 += 64) {
-            uint32_t r0[32], r1[32];
-            tm_ld32(s_addr + c0, r0);
-            tm_ld32(s_addr + c0 + 32, r1);
-            tm_ld_wait();
-            const uint32_t v0 = !tail ? 0xffffffffu : used ? tree_visible(s0 + c0, sq.len, bits) : 0u;
-            const uint32_t v1 = !tail ? 0xffffffffu : used ? tree_visible(s0 + c0 + 32, sq.len, bits) : 0u;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t p16[16];
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                float p[4];
-                if constexpr (Z::CODED) {
-                  const int at = c0 + 32 * h + j;
-                  const float4 kk = *reinterpret_cast<const float4*>(sc + at), lv = *reinterpret_cast<const float4*>(sc + KT + at),
-                               iv = *reinterpret_cast<const float4*>(sc + 2 * KT + at);
-                  const float kx[4] = {kk.x, kk.y, kk.z, kk.w}, lx[4] = {lv.x, lv.y, lv.z, lv.w}, ix[4] = {iv.x, iv.y, iv.z, iv.w};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    const float s = __uint_as_float(h ? r1[j + e] : r0[j + e]);
-                    p[e] = tm_exp2(fmaf(s, kx[e], lx[e]) - base);
-                    if (tail && !(((h ? v1 : v0) >> (j + e)) & 1u)) p[e] = 0.f;
-                    if (tail && p[e] == 0.f) continue;  // 1 / v_scale may be infinite where it is not seen
-                    (e & 1 ? l1 : l0) = fmaf(p[e], ix[e], e & 1 ? l1 : l0);
-                  }
-                } else {
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    p[e] = tm_exp2(fmaf(__uint_as_float(h ? r1[j + e] : r0[j + e]), c, -base));
-                    if (tail && !(((h ? v1 : v0) >> (j + e)) & 1u)) p[e] = 0.f;
-                    (e & 1 ? l1 : l0) += p[e];
-                  }
-                }
-                p16[j / 2] = tm_pack<T>(p[0], p[1]);
-                p16[j / 2 + 1] = tm_pack<T>(p[2], p[3]);
-              }
-              tm_st16(s_addr + (c0 + 32 * h) / 2, p16);
-            }
-          }
-          l += l0 + l1;
+          l += tail ? tm_row_weights<T, STORE, true>(r, s_addr, sc, c, base) : tm_row_weights<T, STORE, false>(r, s_addr, sc, c, base);
           tm_st_wait();
           tm_fence_before();
         }
         __syncwarp();
-        if (lane == 0) tm_arrive(&p_full[st]);
+        if (lane == 0) tm_arrive(&p_full[2 * st + buf]);
       }
       // ---- the segment's end
       const bool have = nt > st;
       bool ok = true;
-      if (have) {
-        ok = tm_wait(&o_full[st], n_o & 1, dead);
-        ++n_o;
-      }
+      if (have) ok = tm_wait(&o_full[st], n_o++ & 1, dead);  // (pv_done may be one phase or two behind or ahead here: its parity says nothing)
       ok = __all_sync(0xffffffffu, ok);
       tm_fence_after();
       if (!used) {  // whatever a row that is not in use has gathered next to others
@@ -488,6 +520,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         ml_s[st * 2 * TM_ROWS + row] = m;
         ml_s[(st * 2 + 1) * TM_ROWS + row] = l;
       }
+      __syncwarp();
       asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");  // m, l and bad_s of all warps; every product of the segment is done
       if (NS == 2) {
         const float mo = ml_s[(st ^ 1) * 2 * TM_ROWS + row], lo = ml_s[((st ^ 1) * 2 + 1) * TM_ROWS + row];
@@ -497,94 +530,100 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         l = l * f + lo * fo;
       }
       const bool gone = !ok || *dead;
-      const bool both = NS == 2 && nt > 1;
       const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
-      const long long slot = 2 * cta + (w.x == begin ? 0 : 1);
+      const int slot = 2 * cta + (w.x == begin ? 0 : 1);
       float* po = tree_part_o(a, TM_ROWS, slot);
       float* xch = reinterpret_cast<float*>(q_t);  // [columns][rows]: no product reads Q any more
       const unsigned long long bad = bad_s & bits;
       T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + tok * a.o_tok + head * a.o_head;
       const float inv = big == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-      constexpr int HALF = HD / 2;
+      // Two streams: each finishes half of the columns, QW at a time, and hands the other its part of them.
+      constexpr int QW = NS == 2 ? HD / 4 : 16, ROUNDS = NS == 2 ? 2 : HD / 16;
 #pragma unroll 1
-      for (int part = 0; part < 2; ++part) {
-        if (both && st == 1) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < HALF; c0 += 32) {
-            uint32_t r[32];
-            tm_ld32(o_addr + part * HALF + c0, r);
-            tm_ld_wait();
+      for (int q = 0; q < ROUNDS; ++q) {
+        const int col = (NS == 2 ? st * (HD / 2) : 0) + q * QW;
+        if (NS == 2 && nt > 1) {
+          if (warp_used) {
+            const int give = (st ^ 1) * (HD / 2) + q * QW;
+            float* to = xch + st * (QW * TM_ROWS) + row;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) xch[(c0 + j) * TM_ROWS + row] = __uint_as_float(r[j]) * f;
+            for (int c0 = 0; c0 < QW; c0 += 16) {
+              uint32_t r[16];
+              tm_ld16(o_addr + give + c0, r);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) to[(c0 + j) * TM_ROWS] = __uint_as_float(r[j]) * f;
+            }
+          }
+        } else if (NS == 2 && st == 0 && warp_used) {  // one tile: stream 1 has nothing, and its half comes from stream 0
+          float* to = xch + row;
+#pragma unroll
+          for (int c0 = 0; c0 < QW; c0 += 16) {
+            uint32_t r[16];
+            tm_ld16(o_addr + HD / 2 + q * QW + c0, r);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) to[(c0 + j) * TM_ROWS] = __uint_as_float(r[j]) * f;
           }
         }
-        if (both) asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");
-        if (st == 0 && warp_used) {
+        __syncwarp();
+        if (NS == 2) asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");
+        if (warp_used) {
+          const float* from = xch + (st ^ 1) * (QW * TM_ROWS) + row;
 #pragma unroll 1
-          for (int c0 = 0; c0 < HALF; c0 += 32) {
-            const int col = part * HALF + c0;
-            uint32_t r[32];
-            tm_ld32(o_addr + col, r);
-            tm_ld_wait();
-            float o[32];
+          for (int c0 = 0; c0 < QW; c0 += 16) {
+            float o[16];
+            if (have) {
+              uint32_t r[16];
+              tm_ld16(o_addr + col + c0, r);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              o[j] = __uint_as_float(r[j]) * f;
-              if (both) o[j] += xch[(c0 + j) * TM_ROWS + row];
-              if (big == -INFINITY && l == 0.f) o[j] = 0.f;  // nothing seen: what the weights of zero met does not count
+              for (int j = 0; j < 16; ++j) o[j] = __uint_as_float(r[j]) * f;
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = 0.f;
             }
-            if (bad) {  // values that are not finite, for the rows that see them
-              for (unsigned long long left = bad; left; left &= left - 1) {
-                const int node = __ffsll(static_cast<long long>(left)) - 1;
-                const auto* vr = vc.row(sg.b, sg.head, sq.len + node);
-#pragma unroll 1
-                for (int j = 0; j < 32; ++j)
-                  if (col + j < a.hd) {
-                    const float v = held_value<T, STORE>(vr[col + j], 1.f);
-                    if (!isfinite(v)) {
+            if (NS == 2 && (nt > 1 || st == 1)) {
 #pragma unroll
-                      for (int k = 0; k < 32; ++k)
-                        if (k == j) o[k] += v;
-                    }
-                  }
-              }
+              for (int j = 0; j < 16; ++j) o[j] += from[(c0 + j) * TM_ROWS];
             }
-            if (gone) {
+            // Nothing seen: what weights of zero met does not count.  A wait that expired: not a number.
+            if (gone || (big == -INFINITY && l == 0.f)) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __int_as_float(0x7fc00000);
+              for (int j = 0; j < 16; ++j) o[j] = gone ? __int_as_float(0x7fc00000) : 0.f;
             }
             if (whole) {
               if (mine) {
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                  if (col + j < a.hd) {
-                    uint4 v;
-                    v.x = tm_pack<T>(o[j] * inv, o[j + 1] * inv), v.y = tm_pack<T>(o[j + 2] * inv, o[j + 3] * inv);
-                    v.z = tm_pack<T>(o[j + 4] * inv, o[j + 5] * inv), v.w = tm_pack<T>(o[j + 6] * inv, o[j + 7] * inv);
-                    if (vec) {
-                      st16(dst + col + j, v);
-                    } else {
-                      const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-                      for (int k = 0; k < 8; ++k) dst[col + j + k] = e[k];
-                    }
-                  }
-                }
+                for (int j = 0; j < 16; j += 8)
+                  if (col + c0 + j < a.hd)
+                    tm_store8(dst + col + c0 + j, vec,
+                              make_uint4(tm_pack<T>(o[j] * inv, o[j + 1] * inv), tm_pack<T>(o[j + 2] * inv, o[j + 3] * inv),
+                                         tm_pack<T>(o[j + 4] * inv, o[j + 5] * inv), tm_pack<T>(o[j + 6] * inv, o[j + 7] * inv)));
               }
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; j += 4)
-                if (col + j < a.hd)
-                  *reinterpret_cast<float4*>(po + (static_cast<size_t>((col + j) / 4) * TM_ROWS + row) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+              for (int j = 0; j < 16; j += 4)
+                if (col + c0 + j < a.hd)
+                  *reinterpret_cast<float4*>(po + (static_cast<size_t>((col + c0 + j) / 4) * TM_ROWS + row) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
             __syncwarp();
           }
-        } else if (st == 0 && whole && mine) {  // a warp of rows that are not in use: zeros
-          for (int j = part * HALF; j < min(a.hd, (part + 1) * HALF); ++j) dst[j] = DT<T>::from_f(0.f);
+        } else if (whole && mine) {  // a warp of rows that are not in use: zeros
+          for (int j = col; j < min(a.hd, col + QW); ++j) dst[j] = DT<T>::from_f(0.f);
         }
         __syncwarp();
-        if (both) asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");
+        if (NS == 2) asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");
       }
+      if (bad && !gone) {  // values that are not finite, for the rows that see them
+        for (unsigned long long left = bad; left; left &= left - 1) {
+          const auto* vr = vc.row(sg.b, sg.head, sq.len + __ffsll(static_cast<long long>(left)) - 1);
+          for (int d = st * (HD / 2); d < min(a.hd, NS == 2 ? (st + 1) * (HD / 2) : HD); ++d) {  // the columns that this thread has written
+            const float v = held_value<T, STORE>(vr[d], 1.f);
+            if (isfinite(v)) continue;
+            if (whole) dst[d] = DT<T>::from_f(DT<T>::to_f(dst[d]) + v);
+            else po[(static_cast<size_t>(d / 4) * TM_ROWS + row) * 4 + d % 4] += v;
+          }
+        }
+      }
+      __syncwarp();
       if (st == 0 && !whole) {
         float* ml = tree_part_ml(a, TM_ROWS, slot);
         ml[row] = big;
@@ -598,7 +637,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     }
   } else if (warp == 4 * NS) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    {
       uint32_t nk = 0;  // 16-bit: tiles; codes: K and V tiles in turn
       bool ok = true;
       while (ok && tm_next_segment(a, line, pre, w)) {
@@ -608,22 +647,28 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
             for (int half = 0; half < 2 && ok; ++half) {
               const uint32_t d = half ? DV : DK, s = nk % d, use = nk / d;
               uint64_t *full = half ? &v_full[s] : &k_full[s], *empty = half ? &v_empty[s] : &k_empty[s];
-              if (use) ok = tm_wait(empty, (use - 1) & 1, dead);
+              if (use) ok = __all_sync(0xffffffffu, tm_wait(empty, (use - 1) & 1, dead));
               if (!ok) break;
-              mbar_expect_tx(full, Z::TILE);
               unsigned char* dst = (half ? v_t : k_t) + s * Z::TILE;
+              if (tm_elect()) {
+                mbar_expect_tx(full, Z::TILE);
 #pragma unroll
-              for (int i = 0; i < Z::BOXES; ++i)
-                tm_load(dst + i * Z::BOX, half ? &maps.v : &maps.k, maps.order, 64 * i, s0, w.sg.head, w.sg.b, full);
+                for (int i = 0; i < Z::BOXES; ++i)
+                  tm_load(dst + i * Z::BOX, half ? &maps.v : &maps.k, maps.order, 64 * i, s0, w.sg.head, w.sg.b, full);
+              }
+              __syncwarp();
             }
             if (ok) ++nk;
           } else {
             for (int half = 0; half < 2 && ok; ++half) {
               const uint32_t s = nk % Z::RAW, use = nk / Z::RAW;
-              if (use) ok = tm_wait(&raw_empty[s], (use - 1) & 1, dead);
+              if (use) ok = __all_sync(0xffffffffu, tm_wait(&raw_empty[s], (use - 1) & 1, dead));
               if (!ok) break;
-              mbar_expect_tx(&raw_full[s], Z::RAW_TILE);
-              tm_load(raw_t + s * Z::RAW_TILE, half ? &maps.v : &maps.k, maps.order, 0, s0, w.sg.head, w.sg.b, &raw_full[s]);
+              if (tm_elect()) {
+                mbar_expect_tx(&raw_full[s], Z::RAW_TILE);
+                tm_load(raw_t + s * Z::RAW_TILE, half ? &maps.v : &maps.k, maps.order, 0, s0, w.sg.head, w.sg.b, &raw_full[s]);
+              }
+              __syncwarp();
               ++nk;
             }
           }
@@ -641,64 +686,70 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         }
       }
     }
-  } else if (warp == 4 * NS + 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+  } else if (warp <= 4 * NS + Z::ISSUERS) {
+    // ------------------------------------------------------------------ a stream's products
+    {
       constexpr uint32_t fmt = DT<T>::id == STX_BF16 ? 1u : 0u;
       constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(TM_ROWS >> 4) << 24);
       constexpr uint32_t idesc_s = common | (static_cast<uint32_t>(KT >> 3) << 17);
       constexpr uint32_t idesc_o = common | (1u << 16) | (static_cast<uint32_t>(HD >> 3) << 17);  // V is MN-major
-      const int ksteps = (a.hd + 15) / 16;  // values of a head behind hd are zeros
-      uint32_t segs = 0, np[2] = {0, 0};
+      const int st = warp - (4 * NS + 1);
+      uint32_t segs = 0, taken[2] = {0, 0};  // segments; uses of the stream's two P buffers
       uint32_t tiles = 0;
       bool ok = true;
+      const uint64_t dq = tm_desc(smem_u32(q_t), 16);
       auto issue_s = [&](int i) {
-        const uint32_t n = tiles + i;
-        const int s = static_cast<int>(n % DK), st = i % NS;
-        if (!tm_wait(&k_full[s], (n / DK) & 1, dead)) return false;
+        const uint32_t n = tiles + i, s = n % DK, b = 2 * st + ((i / NS) & 1);
+        if (!__all_sync(0xffffffffu, tm_wait(&k_full[s], (n / DK) & 1, dead))) return false;
         tm_fence_after();
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t qa = smem_u32(q_t) + (k >> 2) * Z::QBOX + (k & 3) * 32, ka = smem_u32(k_t) + s * Z::TILE + (k >> 2) * Z::BOX + (k & 3) * 32;
-          tm_mma_ss(tmem + st * Z::S_COLS, tm_desc(qa, 16), tm_desc(ka, 16), idesc_s, k != 0);
+        const uint64_t dk = tm_desc(smem_u32(k_t) + s * Z::TILE, 16);
+        if (tm_elect()) {
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)  // values behind head_dim are zeros.  (Skipped by a branch here, all steps came out with the first one's A.)
+            tm_mma_ss(tmem + b * KT, dq + ((k >> 2) * Z::QBOX + (k & 3) * 32) / 16, dk + ((k >> 2) * Z::BOX + (k & 3) * 32) / 16, idesc_s, k != 0);
+          tm_commit(&k_empty[s]);
+          tm_commit(&s_full[b]);
         }
-        tm_commit(&k_empty[s]);
-        tm_commit(&s_full[st]);
+        __syncwarp();
         return true;
       };
       while (ok && tm_next_segment(a, line, pre, w)) {
         const int nt = w.sg.t1 - w.sg.t0;
-        ok = tm_wait(q_full, segs & 1, dead);
+        ok = __all_sync(0xffffffffu, tm_wait(q_full, segs & 1, dead));
         ++segs;
         tm_fence_after();
-        for (int i = 0; i < min(NS, nt) && ok; ++i) ok = issue_s(i);
-        for (int i = 0; i < nt && ok; ++i) {
-          const uint32_t n = tiles + i;
-          const int s = static_cast<int>(n % DV), st = i % NS;
-          ok = tm_wait(&p_full[st], np[st] & 1, dead) && tm_wait(&v_full[s], (n / DV) & 1, dead);
+        for (int i = st; i < min(NB, nt) && ok; i += NS) ok = issue_s(i);
+        for (int i = st; i < nt && ok; i += NS) {
+          const uint32_t n = tiles + i, s = n % DV, half = (i / NS) & 1, b = 2 * st + half;
+          const uint32_t use = half ? taken[1]++ : taken[0]++;
+          ok = tm_wait(&p_full[b], use & 1, dead) && tm_wait(&v_full[s], (n / DV) & 1, dead);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          ++np[st];
           tm_fence_after();
-          const uint32_t va = smem_u32(v_t) + s * Z::TILE;
+          const uint64_t dv = tm_desc(smem_u32(v_t) + s * Z::TILE, Z::BOX);
+          if (tm_elect()) {
 #pragma unroll
-          for (int k = 0; k < KT / 16; ++k)
-            tm_mma_ts(tmem + Z::O_COL + st * HD, tmem + st * Z::S_COLS + k * 8, tm_desc(va + k * 2048, Z::BOX), idesc_o, i >= NS || k != 0);
-          tm_commit(&v_empty[s]);
-          if (i + NS >= nt) tm_commit(&o_full[st]);
-          if (i + NS < nt) {
-            ok = tm_wait(&v_empty[s], (n / DV) & 1, dead);  // P is read: S may overwrite it
-            if (ok) ok = issue_s(i + NS);
+            for (int k = 0; k < KT / 16; ++k)
+              tm_mma_ts(tmem + Z::O_COL + st * HD, tmem + b * KT + k * 8, dv + k * 2048 / 16, idesc_o, i >= NS || k != 0);
+            tm_commit(&v_empty[s]);
+            tm_commit(&pv_done[st]);
+            if (i + NS >= nt) tm_commit(&o_full[st]);
           }
+          __syncwarp();
+          // the next S of this buffer goes over the P just taken; the soft-max works on the other buffer meanwhile
+          if (i + NB < nt) ok = __all_sync(0xffffffffu, tm_wait(&v_empty[s], (n / DV) & 1, dead)) && issue_s(i + NB);
         }
         tiles += nt;
       }
       if (*dead) {  // no product may still be running when tensor memory is freed
-        tm_commit(drain);
-        mbar_wait_bounded(drain, 0);
+        if (tm_elect()) tm_commit(&drain[st]);
+        __syncwarp();
+        mbar_wait_bounded(&drain[st], 0);
       }
     }
   } else if constexpr (Z::CODED) {
     // ------------------------------------------------------------------ codes become operands
-    const int ct = tid - 32 * (4 * NS + 2);  // 0 .. 127
+    const int ct = tid - 32 * (4 * NS + 1 + Z::ISSUERS);  // 0 .. 127
     const float c = fabsf(a.scale_log2);
     uint32_t nr = 0;  // K and V tiles in turn
     uint32_t n = 0;
