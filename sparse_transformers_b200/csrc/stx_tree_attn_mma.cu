@@ -43,22 +43,22 @@ template <int STORE, int HD> struct TmShape {
   static constexpr uint32_t BOX = KT * 128;         // bytes of such a part of a K or V tile
   static constexpr uint32_t TILE = BOXES * BOX;
   static constexpr uint32_t QBOX = TM_ROWS * 128, Q = BOXES * QBOX;
-  // Tiles in shared memory (16-bit).  K runs ahead of V by the S that are formed in advance.  What an SM has to have on its way is 45 KB
-  // (0.3 KB/ns of HBM x 148 SMs at 1 us).
-  static constexpr int DK = HD == 64 ? (CODED ? 6 : 8) : HD == 128 ? (CODED ? 4 : 6) : 2;
-  static constexpr int DV = HD == 64 ? (CODED ? 4 : 6) : HD == 128 ? (CODED ? 3 : 5) : CODED ? 1 : 2;
-  static constexpr int RAW = CODED ? (HD == 64 ? 12 : HD == 128 ? 8 : 3) : 0;  // tiles of codes, K and V in turn
+  // Tiles in shared memory (16-bit), in a ring for each stream: whoever waits for a slot then knows its ring's earlier phases to be over, and
+  // a phase's parity is not taken for another's.  What an SM has to have on its way is 45 KB (0.3 KB/ns of HBM x 148 SMs at 1 us).
+  static constexpr int DK = HD == 64 ? (CODED ? 3 : 4) : HD == 128 ? (CODED ? 2 : 3) : 2;
+  static constexpr int DV = HD == 64 ? (CODED ? 2 : 3) : HD == 128 ? 2 : CODED ? 1 : 2;
+  static constexpr int RAW = CODED ? (HD == 64 ? 6 : HD == 128 ? 3 : 1) : 0;  // tiles of codes of K, and as many of V
   static constexpr uint32_t RAW_TILE = KT * HD;
-  // Tiles whose scales are kept: those of tile n are overwritten with K of tile n + SCALES, which waits for S of tile n + SCALES - DK = n + NB,
-  // the next S in the buffer of tile n, and so for the P of tile n.
-  static constexpr int SCALES = DK + NB;
+  // Tiles of a stream whose scales are kept: those of tile c are overwritten with K of tile c + SCALES, which waits for S of tile c + 2, formed
+  // in the place of P of tile c.
+  static constexpr int SCALES = DK + 2;
   static constexpr int ISSUERS = NS;                // warps that issue products, one for each stream
-  static constexpr int WARPS = 4 * NS + 1 + ISSUERS + (CODED ? 4 : 0);
+  static constexpr int WARPS = 4 * NS + 2 + ISSUERS + (CODED ? 4 : 0);
   static constexpr int THREADS = 32 * WARPS;
   static constexpr uint32_t O_COL = 256;
-  static constexpr uint32_t SMEM_TILES = Q + DK * TILE + DV * TILE + RAW * RAW_TILE;
-  static constexpr uint32_t SMEM_SCALES = CODED ? SCALES * 3 * KT * 4 : 0;
-  static constexpr uint32_t BARS = 2 * DK + 2 * DV + 2 * NB + 2 * NS + 1 + NS + 2 * RAW + (CODED ? SCALES : 0);
+  static constexpr uint32_t SMEM_TILES = Q + NS * (DK + DV) * TILE + 2 * RAW * RAW_TILE;
+  static constexpr uint32_t SMEM_SCALES = CODED ? NS * SCALES * 3 * KT * 4 : 0;
+  static constexpr uint32_t BARS = 2 * NS * (DK + DV) + 2 * NB + 4 * NS + 4 * RAW + (CODED ? NS * SCALES : 0);
   static constexpr uint32_t SMEM = 1024 + SMEM_TILES + SMEM_SCALES + 2 * 2 * TM_ROWS * 4 + BARS * 8 + 64;
   static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1) + 64 <= 227 * 1024, "shared memory of a CTA");
 };
@@ -328,24 +328,24 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* q_t = smem;
   unsigned char* k_t = q_t + Z::Q;
-  unsigned char* v_t = k_t + DK * Z::TILE;
-  unsigned char* raw_t = v_t + DV * Z::TILE;
-  float* sc_s = reinterpret_cast<float*>(raw_t + Z::RAW * Z::RAW_TILE);  // [SCALES][3][KT]
+  unsigned char* v_t = k_t + NS * DK * Z::TILE;
+  unsigned char* raw_t = v_t + NS * DV * Z::TILE;
+  float* sc_s = reinterpret_cast<float*>(raw_t + 2 * Z::RAW * Z::RAW_TILE);  // [SCALES][3][KT]
   float* ml_s = sc_s + Z::SMEM_SCALES / 4;                               // [2][2][TM_ROWS]
   uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + 2 * 2 * TM_ROWS);
-  uint64_t *k_full = bars, *k_empty = k_full + DK, *v_full = k_empty + DK, *v_empty = v_full + DV, *s_full = v_empty + DV;
-  uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + 1, *raw_full = drain + NS;
-  uint64_t *raw_empty = raw_full + Z::RAW, *sc_full = raw_empty + Z::RAW;
+  uint64_t *k_full = bars, *k_empty = k_full + NS * DK, *v_full = k_empty + NS * DK, *v_empty = v_full + NS * DV, *s_full = v_empty + NS * DV;
+  uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + NS, *raw_full = drain + NS;
+  uint64_t *raw_empty = raw_full + 2 * Z::RAW, *sc_full = raw_empty + 2 * Z::RAW;  // K's, then V's
   volatile int* dead = &dead_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (tid == 0) {
-    for (int i = 0; i < DK; ++i) {
-      mbar_init(&k_full[i], Z::CODED ? 4 : 1);
+    for (int i = 0; i < NS * DK; ++i) {
+      mbar_init(&k_full[i], Z::CODED ? 2 : 1);
       mbar_init(&k_empty[i], 1);
     }
-    for (int i = 0; i < DV; ++i) {
-      mbar_init(&v_full[i], Z::CODED ? 4 : 1);
+    for (int i = 0; i < NS * DV; ++i) {
+      mbar_init(&v_full[i], Z::CODED ? 2 : 1);
       mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < NB; ++i) {
@@ -356,14 +356,14 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&drain[i], 1);
+      mbar_init(&q_full[i], 4 * NS);
     }
-    mbar_init(q_full, 4 * NS);
-    for (int i = 0; i < Z::RAW; ++i) {
+    for (int i = 0; i < 2 * Z::RAW; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 4);
+      mbar_init(&raw_empty[i], 2);
     }
     if (Z::CODED)
-      for (int i = 0; i < Z::SCALES; ++i) mbar_init(&sc_full[i], 4);
+      for (int i = 0; i < NS * Z::SCALES; ++i) mbar_init(&sc_full[i], 2);
     dead_s = 0;
     bad_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -375,7 +375,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   const TreeLine line = tree_line(a, pre);
   const int cta = blockIdx.x;
   if (cta >= line.ctas) return;
-  if (warp == 4 * NS + 1) {
+  if (warp == 4 * NS + 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_s)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -388,6 +388,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   w.x = begin;
   w.end = tree_begin(line, cta + 1);
   w.begun = false;
+  uint32_t issued[2] = {0, 0};  // copies that a producer has requested, by ring
 
   if (warp < 4 * NS) {
     // ------------------------------------------------------------------ softmax: a thread has a row
@@ -397,7 +398,6 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     const float c = fabsf(a.scale_log2);
     uint32_t uses[2] = {0, 0};  // of the stream's two S buffers
     uint32_t n_o = 0;           // segments in which the stream had a tile
-    uint32_t tiles = 0;         // tiles of the CTA before this segment
     while (tm_next_segment(a, line, pre, w)) {
       const TreeSeg& sg = w.sg;
       const TreeSeq& sq = w.sq;
@@ -407,6 +407,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       const bool used = mine && tok < sq.cnt;
       const unsigned long long bits = used ? tree_bits(a, sq, sg.b, tok) : 0ull;
       const bool warp_used = __any_sync(0xffffffffu, used);
+      const int nt = sg.t1 - sg.t0;
       // ---- Q: each of the NS warps of a lane group brings a part of the rows' boxes
       {
         const T* src = static_cast<const T*>(a.q) + sg.b * a.q_seq + tok * a.q_tok + head * a.q_head;
@@ -429,26 +430,30 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         }
         tm_fence_async();
         __syncwarp();
-        if (lane == 0) tm_arrive(q_full);
+        if (lane == 0) {  // a stream without a tile is not told: its phases are those of segments that cannot end without it
+          tm_arrive(&q_full[0]);
+          if (NS == 2 && nt > 1) tm_arrive(&q_full[1]);
+        }
       }
       float m = -INFINITY, l = 0.f;
-      const int nt = sg.t1 - sg.t0;
       for (int i = st; i < nt; i += NS) {
         const int s0 = (sg.t0 + i) * KT, buf = (i / NS) & 1;
         const bool tail = s0 + KT > sq.len;
-        const uint32_t n = tiles + i;
+        const uint32_t n = uses[0] + uses[1];  // tiles of this stream before this one
         const uint32_t s_addr = s_base + buf * KT;
-        const float* sc = sc_s + (Z::CODED ? (n % Z::SCALES) * 3 * KT : 0);
+        const uint32_t ss = Z::CODED ? st * Z::SCALES + n % Z::SCALES : 0;
+        const float* sc = sc_s + ss * 3 * KT;
         const uint32_t use = buf ? uses[1]++ : uses[0]++;
         bool ok = tm_wait(&s_full[2 * st + buf], use & 1, dead);
-        if (Z::CODED) ok = tm_wait(&sc_full[n % Z::SCALES], (n / Z::SCALES) & 1, dead) && ok;
+        if (Z::CODED) ok = tm_wait(&sc_full[ss], (n / Z::SCALES) & 1, dead) && ok;
         if (tail) {
           // slots behind the keys become zeros, and what is not finite in a node's value: 0 * NaN must not reach a row that
           // does not see the node (those that do get it back at the end)
-          ok = tm_wait(&v_full[n % DV], (n / DV) & 1, dead) && ok;
+          if (DV < 2 && i >= NS) ok = tm_wait(&pv_done[st], (n - 1) & 1, dead) && ok;  // else the slot's phase before may still be open
+          ok = tm_wait(&v_full[st * DV + n % DV], (n / DV) & 1, dead) && ok;
           const int r = tid & 127, slot = s0 + r;
           if (ok && r < KT && slot >= sq.len) {
-            unsigned char* vr = v_t + (n % DV) * Z::TILE + r * 128;
+            unsigned char* vr = v_t + (st * DV + n % DV) * Z::TILE + r * 128;
             bool bad = false;
 #pragma unroll 1
             for (int ch = 0; ch < HD / 8; ++ch) {
@@ -484,8 +489,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
             l *= f;
             if (i >= NS) {  // O holds something: the stream's last product has to be in it
               // Phase by parity: the one before it is over since S of this tile was formed, the one behind it waits for this tile's P.
-              const uint32_t done = uses[0] + uses[1] - 2;
-              ok = __all_sync(0xffffffffu, tm_wait(&pv_done[st], done & 1, dead));
+              ok = __all_sync(0xffffffffu, tm_wait(&pv_done[st], (n - 1) & 1, dead));
               tm_fence_after();
 #pragma unroll 1
               for (int c0 = 0; c0 < HD; c0 += 16) {
@@ -633,74 +637,50 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       __syncwarp();
       asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");  // Q and bad_s are free
       if (tid == 0) bad_s = 0;
-      tiles += nt;
     }
-  } else if (warp == 4 * NS) {
-    // ------------------------------------------------------------------ TMA producer
-    {
-      uint32_t nk = 0;  // 16-bit: tiles; codes: K and V tiles in turn
-      bool ok = true;
-      while (ok && tm_next_segment(a, line, pre, w)) {
-        for (int t = w.sg.t0; t < w.sg.t1 && ok; ++t) {
-          const int s0 = t * KT;
-          if constexpr (!Z::CODED) {
-            for (int half = 0; half < 2 && ok; ++half) {
-              const uint32_t d = half ? DV : DK, s = nk % d, use = nk / d;
-              uint64_t *full = half ? &v_full[s] : &k_full[s], *empty = half ? &v_empty[s] : &k_empty[s];
-              if (use) ok = __all_sync(0xffffffffu, tm_wait(empty, (use - 1) & 1, dead));
-              if (!ok) break;
-              unsigned char* dst = (half ? v_t : k_t) + s * Z::TILE;
-              if (tm_elect()) {
-                mbar_expect_tx(full, Z::TILE);
+  } else if (warp < 4 * NS + 2) {
+    // ------------------------------------------------------------------ TMA producers: one for K, one for V (a warp issues a box in about 150 ns)
+    const int half = warp - 4 * NS;
+    const CUtensorMap* map = half ? &maps.v : &maps.k;
+    constexpr uint32_t BYTES = Z::CODED ? Z::RAW_TILE : Z::TILE;
+    const uint32_t d = Z::CODED ? Z::RAW : half ? DV : DK;
+    uint64_t* full = Z::CODED ? raw_full + half * Z::RAW : half ? v_full : k_full;
+    uint64_t* empty = Z::CODED ? raw_empty + half * Z::RAW : half ? v_empty : k_empty;
+    unsigned char* base = Z::CODED ? raw_t + half * Z::RAW * Z::RAW_TILE : half ? v_t : k_t;
+    uint32_t n[2] = {0, 0};  // tiles of each ring so far (codes: one ring for both streams)
+    bool ok = true;
+    while (ok && tm_next_segment(a, line, pre, w)) {
+      for (int t = w.sg.t0; t < w.sg.t1 && ok; ++t) {
+        const uint32_t st = Z::CODED || NS == 1 ? 0 : (t - w.sg.t0) & 1;
+        const uint32_t m = st ? n[1]++ : n[0]++, use = m / d, s = st * d + m % d;
+        if (use) ok = __all_sync(0xffffffffu, tm_wait(&empty[s], (use - 1) & 1, dead));
+        if (!ok) break;
+        if (tm_elect()) {
+          mbar_expect_tx(&full[s], BYTES);
 #pragma unroll
-                for (int i = 0; i < Z::BOXES; ++i)
-                  tm_load(dst + i * Z::BOX, half ? &maps.v : &maps.k, maps.order, 64 * i, s0, w.sg.head, w.sg.b, full);
-              }
-              __syncwarp();
-            }
-            if (ok) ++nk;
-          } else {
-            for (int half = 0; half < 2 && ok; ++half) {
-              const uint32_t s = nk % Z::RAW, use = nk / Z::RAW;
-              if (use) ok = __all_sync(0xffffffffu, tm_wait(&raw_empty[s], (use - 1) & 1, dead));
-              if (!ok) break;
-              if (tm_elect()) {
-                mbar_expect_tx(&raw_full[s], Z::RAW_TILE);
-                tm_load(raw_t + s * Z::RAW_TILE, half ? &maps.v : &maps.k, maps.order, 0, s0, w.sg.head, w.sg.b, &raw_full[s]);
-              }
-              __syncwarp();
-              ++nk;
-            }
-          }
+          for (int i = 0; i < (Z::CODED ? 1 : Z::BOXES); ++i)
+            tm_load(base + s * BYTES + i * Z::BOX, map, maps.order, 64 * i, t * KT, w.sg.head, w.sg.b, &full[s]);
         }
-      }
-      if (*dead) {  // no copy may still be on its way when the CTA leaves
-        if constexpr (!Z::CODED) {
-          for (uint32_t s = 0; s < DK; ++s)
-            if (nk > s) mbar_wait_bounded(&k_full[s], ((nk - 1 - s) / DK) & 1);
-          for (uint32_t s = 0; s < DV; ++s)
-            if (nk > s) mbar_wait_bounded(&v_full[s], ((nk - 1 - s) / DV) & 1);
-        } else {
-          for (uint32_t s = 0; s < Z::RAW; ++s)
-            if (nk > s) mbar_wait_bounded(&raw_full[s], ((nk - 1 - s) / Z::RAW) & 1);
-        }
+        __syncwarp();
+        issued[0] = n[0], issued[1] = n[1];
       }
     }
-  } else if (warp <= 4 * NS + Z::ISSUERS) {
+  } else if (warp < 4 * NS + 2 + Z::ISSUERS) {
     // ------------------------------------------------------------------ a stream's products
     {
       constexpr uint32_t fmt = DT<T>::id == STX_BF16 ? 1u : 0u;
       constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(TM_ROWS >> 4) << 24);
       constexpr uint32_t idesc_s = common | (static_cast<uint32_t>(KT >> 3) << 17);
       constexpr uint32_t idesc_o = common | (1u << 16) | (static_cast<uint32_t>(HD >> 3) << 17);  // V is MN-major
-      const int st = warp - (4 * NS + 1);
-      uint32_t segs = 0, taken[2] = {0, 0};  // segments; uses of the stream's two P buffers
-      uint32_t tiles = 0;
+      const int st = warp - (4 * NS + 2);
+      uint32_t segs = 0, taken[2] = {0, 0};  // segments with a tile of the stream; uses of the stream's two P buffers
+      uint32_t ns = 0, np = 0;               // S and P V of the stream so far
       bool ok = true;
       const uint64_t dq = tm_desc(smem_u32(q_t), 16);
       auto issue_s = [&](int i) {
-        const uint32_t n = tiles + i, s = n % DK, b = 2 * st + ((i / NS) & 1);
-        if (!__all_sync(0xffffffffu, tm_wait(&k_full[s], (n / DK) & 1, dead))) return false;
+        const uint32_t s = st * DK + ns % DK, b = 2 * st + ((i / NS) & 1);
+        if (!__all_sync(0xffffffffu, tm_wait(&k_full[s], (ns / DK) & 1, dead))) return false;
+        ++ns;
         tm_fence_after();
         const uint64_t dk = tm_desc(smem_u32(k_t) + s * Z::TILE, 16);
         if (tm_elect()) {
@@ -715,14 +695,15 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       };
       while (ok && tm_next_segment(a, line, pre, w)) {
         const int nt = w.sg.t1 - w.sg.t0;
-        ok = __all_sync(0xffffffffu, tm_wait(q_full, segs & 1, dead));
+        if (nt <= st) continue;
+        ok = __all_sync(0xffffffffu, tm_wait(&q_full[st], segs & 1, dead));
         ++segs;
         tm_fence_after();
         for (int i = st; i < min(NB, nt) && ok; i += NS) ok = issue_s(i);
         for (int i = st; i < nt && ok; i += NS) {
-          const uint32_t n = tiles + i, s = n % DV, half = (i / NS) & 1, b = 2 * st + half;
+          const uint32_t s = st * DV + np % DV, half = (i / NS) & 1, b = 2 * st + half;
           const uint32_t use = half ? taken[1]++ : taken[0]++;
-          ok = tm_wait(&p_full[b], use & 1, dead) && tm_wait(&v_full[s], (n / DV) & 1, dead);
+          ok = tm_wait(&p_full[b], use & 1, dead) && tm_wait(&v_full[s], (np / DV) & 1, dead);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tm_fence_after();
@@ -737,33 +718,32 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           }
           __syncwarp();
           // the next S of this buffer goes over the P just taken; the soft-max works on the other buffer meanwhile
-          if (i + NB < nt) ok = __all_sync(0xffffffffu, tm_wait(&v_empty[s], (n / DV) & 1, dead)) && issue_s(i + NB);
+          if (i + NB < nt) ok = __all_sync(0xffffffffu, tm_wait(&pv_done[st], np & 1, dead)) && issue_s(i + NB);
+          ++np;
         }
-        tiles += nt;
-      }
-      if (*dead) {  // no product may still be running when tensor memory is freed
-        if (tm_elect()) tm_commit(&drain[st]);
-        __syncwarp();
-        mbar_wait_bounded(&drain[st], 0);
       }
     }
   } else if constexpr (Z::CODED) {
-    // ------------------------------------------------------------------ codes become operands
-    const int ct = tid - 32 * (4 * NS + 1 + Z::ISSUERS);  // 0 .. 127
+    // ------------------------------------------------------------------ codes become operands: two warps for K (and the scales), two for V
+    const int half = (warp - (4 * NS + 2 + Z::ISSUERS)) >> 1, ct = (tid & 31) + 32 * ((warp - (4 * NS + 2 + Z::ISSUERS)) & 1);
+    const uint32_t d = half ? DV : DK;
+    uint64_t *full = half ? v_full : k_full, *empty = half ? v_empty : k_empty;
+    uint64_t *r_full = raw_full + half * Z::RAW, *r_empty = raw_empty + half * Z::RAW;
+    const unsigned char* raw = raw_t + half * Z::RAW * Z::RAW_TILE;
+    unsigned char* tiles_t = half ? v_t : k_t;
     const float c = fabsf(a.scale_log2);
-    uint32_t nr = 0;  // K and V tiles in turn
-    uint32_t n = 0;
+    uint32_t n[2] = {0, 0}, rs = 0, ruse = 0;  // tiles of each stream so far; place in the ring of codes
     bool ok = true;
     // the scales of a tile are requested a tile ahead
     TmWalk ahead = w;
-    bool more = tm_next_segment(a, line, pre, ahead);
+    bool more = half == 0 && tm_next_segment(a, line, pre, ahead);
     float ks = 0.f, vs = 0.f;
     auto request = [&]() {
       ks = 0.f;
       vs = 1.f;
       if (!more) return;
       const int slot = ahead.t * KT + ct;
-      if (ct < KT && slot < ahead.sq.keys) {
+      if (slot < ahead.sq.keys) {
         ks = kc.srow(ahead.sg.b, ahead.sg.head)[slot];
         vs = vc.srow(ahead.sg.b, ahead.sg.head)[slot];
       }
@@ -771,36 +751,25 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     };
     request();
     while (ok && tm_next_segment(a, line, pre, w)) {
-      for (int t = w.sg.t0; t < w.sg.t1 && ok; ++t, ++n) {
-        const float ks0 = ks, vs0 = vs == 0.f ? 1.f : vs;  // a row of zeros: any scale
-        request();
-#pragma unroll 1
-        for (int half = 0; half < 2 && ok; ++half, ++nr) {
-          const uint32_t rs = nr % Z::RAW;
-          const uint32_t d = half ? DV : DK, s = n % d;
-          const uint32_t use = n / d;
-          if (use) ok = tm_wait(half ? &v_empty[s] : &k_empty[s], (use - 1) & 1, dead);
-          ok = ok && tm_wait(&raw_full[rs], (nr / Z::RAW) & 1, dead);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (half == 0) {
-            float* sc = sc_s + (n % Z::SCALES) * 3 * KT;
-            if (ct < KT) {
-              sc[ct] = ks0 * c;
-              sc[KT + ct] = log2f(vs0);
-              sc[2 * KT + ct] = 1.f / vs0;
-            }
-            __syncwarp();
-            if (lane == 0) tm_arrive(&sc_full[n % Z::SCALES]);
-          }
-          const unsigned char* src = raw_t + rs * Z::RAW_TILE;
-          unsigned char* dst = (half ? v_t : k_t) + s * Z::TILE;
-          constexpr int PER = HD / 16;  // 16-byte pieces of a row of codes
-#pragma unroll 4
-          for (int i = ct; i < KT * PER; i += 128) {
-            const int r = i / PER, piece = i % PER;
-            const uint4 raw = *reinterpret_cast<const uint4*>(src + i * 16);
-            const uint32_t q4[4] = {raw.x, raw.y, raw.z, raw.w};
+      for (int t = w.sg.t0; t < w.sg.t1 && ok; ++t) {
+        const uint32_t st = NS == 1 ? 0 : (t - w.sg.t0) & 1;
+        const uint32_t m = st ? n[1]++ : n[0]++, use = m / d, s = st * d + m % d;
+        if (use) ok = tm_wait(&empty[s], (use - 1) & 1, dead);
+        ok = ok && tm_wait(&r_full[rs], ruse & 1, dead);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        constexpr int PER = HD / 16, EACH = KT * PER / 64;  // 16-byte pieces of a row of codes, of a thread
+        const unsigned char* src = raw + rs * Z::RAW_TILE;
+        unsigned char* dst = tiles_t + s * Z::TILE;
+#pragma unroll
+        for (int i0 = 0; i0 < EACH; i0 += 4) {
+          uint4 w4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w4[i] = *reinterpret_cast<const uint4*>(src + (ct + 64 * (i0 + i)) * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = ct + 64 * (i0 + i), r = at / PER, piece = at % PER;
+            const uint32_t q4[4] = {w4[i].x, w4[i].y, w4[i].z, w4[i].w};
             uint32_t e[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) e[k] = tm_operand<T, STORE>(q4[k / 2], k & 1);
@@ -811,17 +780,32 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
                   if (((q4[k / 4] >> (8 * (k % 4))) & 0x7fu) == 0x7fu) e[k / 2] |= k & 1 ? 0x7fff0000u : 0x00007fffu;
               }
             }
-            unsigned char* at = dst + (piece >> 2) * Z::BOX + r * 128;
+            unsigned char* to = dst + (piece >> 2) * Z::BOX + r * 128;
             const int ch = (piece & 3) * 2;
-            *reinterpret_cast<uint4*>(at + ((ch ^ (r & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
-            *reinterpret_cast<uint4*>(at + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
+            *reinterpret_cast<uint4*>(to + ((ch ^ (r & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+            *reinterpret_cast<uint4*>(to + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
           }
-          tm_fence_async();
+        }
+        tm_fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          tm_arrive(&r_empty[rs]);
+          tm_arrive(&full[s]);
+        }
+        if (half == 0) {
+          const float v = vs == 0.f ? 1.f : vs;  // a row of zeros: any scale
+          const uint32_t ss = st * Z::SCALES + m % Z::SCALES;
+          float* sc = sc_s + ss * 3 * KT;
+          sc[ct] = ks * c;
+          sc[KT + ct] = log2f(v);
+          sc[2 * KT + ct] = 1.f / v;
           __syncwarp();
-          if (lane == 0) {
-            tm_arrive(&raw_empty[rs]);
-            tm_arrive(half ? &v_full[s] : &k_full[s]);
-          }
+          if (lane == 0) tm_arrive(&sc_full[ss]);
+          request();
+        }
+        if (++rs == Z::RAW) {
+          rs = 0;
+          ++ruse;
         }
       }
     }
@@ -829,7 +813,23 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   __syncwarp();
   tm_fence_before();
   __syncthreads();
-  if (warp == 4 * NS + 1) {
+  if (*dead) {  // a wait has expired: no copy and no product may still be on its way when the CTA leaves
+    if (warp >= 4 * NS && warp < 4 * NS + 2) {
+      const int half = warp - 4 * NS;
+      const uint32_t d = Z::CODED ? Z::RAW : half ? DV : DK;
+      uint64_t* full = Z::CODED ? raw_full + half * Z::RAW : half ? v_full : k_full;
+      for (uint32_t st = 0; st < 2; ++st)
+        for (uint32_t i = 0; i < d; ++i)
+          if (issued[st] > i) mbar_wait_bounded(&full[st * d + i], ((issued[st] - 1 - i) / d) & 1);
+    } else if (warp >= 4 * NS + 2 && warp < 4 * NS + 2 + Z::ISSUERS) {
+      const int st = warp - (4 * NS + 2);
+      if (tm_elect()) tm_commit(&drain[st]);
+      __syncwarp();
+      mbar_wait_bounded(&drain[st], 0);
+    }
+    __syncthreads();
+  }
+  if (warp == 4 * NS + 2) {
     tm_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
