@@ -19,8 +19,8 @@
 // both 16-bit types), and the scales of the rows go where they cost nothing: x = S (k_scale c) + log2 v_scale in one fused multiply-add, so that
 // P is the weight times v_scale, bounded by the same running maximum, and l = sum P / v_scale in another.
 //
-// Warps: 4 NS softmax (warp w reads the tensor memory lanes 32 (w mod 4) ..), then the TMA producer, the MMA issuer, and for 8-bit caches
-// four that convert.  Every wait is bounded; when one expires all roles stop waiting, the rows become NaN and tensor memory is freed.
+// Warps: 8 NS softmax (warp w reads the tensor memory lanes 32 (w mod 4) ..), two TMA producers, one that issues the products of each stream, and
+// for 8-bit caches four that convert.  Every wait is bounded; when one expires all roles stop waiting, the rows become NaN and tensor memory is freed.
 #include "stx_tma.cuh"
 #include "stx_tree_attn.cuh"
 
@@ -53,13 +53,15 @@ template <int STORE, int HD> struct TmShape {
   // in the place of P of tile c.
   static constexpr int SCALES = DK + 2;
   static constexpr int ISSUERS = NS;                // warps that issue products, one for each stream
-  static constexpr int WARPS = 4 * NS + 2 + ISSUERS + (CODED ? 4 : 0);
+  static constexpr int SW = 8 * NS;                  // warps of the soft-max: a lane group's rows x two halves of the tile, for each stream
+  static constexpr int WARPS = SW + 2 + ISSUERS + (CODED ? 4 : 0);
   static constexpr int THREADS = 32 * WARPS;
   static constexpr uint32_t O_COL = 256;
   static constexpr uint32_t SMEM_TILES = Q + NS * (DK + DV) * TILE + 2 * RAW * RAW_TILE;
   static constexpr uint32_t SMEM_SCALES = CODED ? NS * SCALES * 3 * KT * 4 : 0;
+  static constexpr uint32_t SMEM_ML = 3 * 2 * NS * TM_ROWS * 4;  // m (of tile and segment) and l of each thread of the soft-max
   static constexpr uint32_t BARS = 2 * NS * (DK + DV) + 2 * NB + 4 * NS + 4 * RAW + (CODED ? NS * SCALES : 0);
-  static constexpr uint32_t SMEM = 1024 + SMEM_TILES + SMEM_SCALES + 2 * 2 * TM_ROWS * 4 + BARS * 8 + 64;
+  static constexpr uint32_t SMEM = 1024 + SMEM_TILES + SMEM_SCALES + SMEM_ML + BARS * 8 + 64;
   static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1) + 64 <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -116,32 +118,35 @@ __device__ __forceinline__ void tm_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 }
 // Columns of the warp's 32 lanes.  The wait is part of the statement: between the two the compiler could move registers that are not
 // there yet (it does where it has to spill).
-__device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tm_ld(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tm_ld(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tm_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+__device__ __forceinline__ void tm_ld(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
 }
@@ -257,61 +262,64 @@ __device__ __forceinline__ void tm_load(void* dst, const CUtensorMap* m, int ord
       : "memory");
 }
 
-// The row's x of a tile from its S (16-bit caches: S itself), what it does not see as -infinity, and the largest of them.  TAIL: the tile has
+// x of 32 slots from their S (16-bit caches: S itself), what the row does not see as -infinity, and the largest of them.  TAIL: there are
 // slots that the row may not see; `cut` is 0 for rows that are not in use.  The two forms are apart so that the common one has no masks in it.
-template <int STORE, bool TAIL>
-__device__ __forceinline__ float tm_row_max(uint32_t (&r)[64], const float* sc, int s0, int len, unsigned long long bits, uint32_t cut) {
+template <int STORE, int KT, bool TAIL>
+__device__ __forceinline__ float tm_row_max(uint32_t (&r)[32], const float* sc, int s0, int len, unsigned long long bits, uint32_t cut) {
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  uint32_t v[2] = {~0u, ~0u};
-  if (TAIL) {
-    v[0] = tree_visible(s0, len, bits) & cut;
-    v[1] = tree_visible(s0 + 32, len, bits) & cut;
-  }
+  const uint32_t v = TAIL ? tree_visible(s0, len, bits) & cut : ~0u;
 #pragma unroll
-  for (int j = 0; j < 64; j += 4) {
+  for (int j = 0; j < 32; j += 4) {
     float x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(r[j + e]);
     if constexpr (STORE != STX_STORE_SAME) {
-      const float4 kk = *reinterpret_cast<const float4*>(sc + j), lv = *reinterpret_cast<const float4*>(sc + 64 + j);
+      const float4 kk = *reinterpret_cast<const float4*>(sc + j), lv = *reinterpret_cast<const float4*>(sc + KT + j);
       x[0] = fmaf(x[0], kk.x, lv.x), x[1] = fmaf(x[1], kk.y, lv.y), x[2] = fmaf(x[2], kk.z, lv.z), x[3] = fmaf(x[3], kk.w, lv.w);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (TAIL) x[e] = (v[j / 32] >> ((j + e) & 31)) & 1u ? x[e] : -INFINITY;
+      if (TAIL) x[e] = (v >> (j + e)) & 1u ? x[e] : -INFINITY;
       mx[e] = fmaxf(mx[e], x[e]);
       r[j + e] = __float_as_uint(x[e]);
     }
   }
   return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
-// P = 2^(x - base), packed in pairs, to the columns from p_addr on; returns the sum of the row's weights.
-template <typename T, int STORE, bool TAIL>
-__device__ __forceinline__ float tm_row_weights(const uint32_t (&r)[64], uint32_t p_addr, const float* sc, float c, float base) {
+// P = 2^(x - base), packed in pairs, to 16 columns from p_addr on; returns the sum of the weights.
+template <typename T, int STORE, int KT, bool TAIL>
+__device__ __forceinline__ float tm_row_weights(const uint32_t (&r)[32], uint32_t p_addr, const float* sc, float c, float base) {
   float l[4] = {0.f, 0.f, 0.f, 0.f};
+  uint32_t p16[16];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t p16[16];
-#pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      float p[4], iv[4] = {1.f, 1.f, 1.f, 1.f};
-      if constexpr (STORE != STX_STORE_SAME) {
-        const float4 ii = *reinterpret_cast<const float4*>(sc + 128 + 32 * h + j);
-        iv[0] = ii.x, iv[1] = ii.y, iv[2] = ii.z, iv[3] = ii.w;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __uint_as_float(r[32 * h + j + e]);
-        p[e] = tm_exp2(STORE != STX_STORE_SAME ? x - base : fmaf(x, c, -base));
-        if (TAIL && x == -INFINITY) p[e] = iv[e] = 0.f;  // not seen: c may be 0, 1 / v_scale infinite or NaN
-        l[e] = STORE != STX_STORE_SAME ? fmaf(p[e], iv[e], l[e]) : l[e] + p[e];
-      }
-      p16[j / 2] = tm_pack<T>(p[0], p[1]);
-      p16[j / 2 + 1] = tm_pack<T>(p[2], p[3]);
+  for (int j = 0; j < 32; j += 4) {
+    float p[4], iv[4] = {1.f, 1.f, 1.f, 1.f};
+    if constexpr (STORE != STX_STORE_SAME) {
+      const float4 ii = *reinterpret_cast<const float4*>(sc + 2 * KT + j);
+      iv[0] = ii.x, iv[1] = ii.y, iv[2] = ii.z, iv[3] = ii.w;
     }
-    tm_st16(p_addr + 16 * h, p16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(r[j + e]);
+      p[e] = tm_exp2(STORE != STX_STORE_SAME ? x - base : fmaf(x, c, -base));
+      if (TAIL && x == -INFINITY) p[e] = iv[e] = 0.f;  // not seen: c may be 0, 1 / v_scale infinite or NaN
+      l[e] = STORE != STX_STORE_SAME ? fmaf(p[e], iv[e], l[e]) : l[e] + p[e];
+    }
+    p16[j / 2] = tm_pack<T>(p[0], p[1]);
+    p16[j / 2 + 1] = tm_pack<T>(p[2], p[3]);
   }
+  tm_st16(p_addr, p16);
   return (l[0] + l[1]) + (l[2] + l[3]);
+}
+// Whether any of the 64 threads of two warps says so; also a barrier of theirs.
+__device__ __forceinline__ bool tm_any64(int bar, bool mine) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %1, 0;\n\tbarrier.cta.red.or.pred b, %2, 64, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<int>(mine)), "r"(bar)
+      : "memory");
+  return r != 0;
 }
 
 template <typename T, int STORE, int HD>
@@ -331,8 +339,8 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   unsigned char* v_t = k_t + NS * DK * Z::TILE;
   unsigned char* raw_t = v_t + NS * DV * Z::TILE;
   float* sc_s = reinterpret_cast<float*>(raw_t + 2 * Z::RAW * Z::RAW_TILE);  // [SCALES][3][KT]
-  float* ml_s = sc_s + Z::SMEM_SCALES / 4;                               // [2][2][TM_ROWS]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + 2 * 2 * TM_ROWS);
+  float* ml_s = sc_s + Z::SMEM_SCALES / 4;  // m of a tile, two in turn [2][2 NS][TM_ROWS] (the first also: m of a segment), l [2 NS][TM_ROWS]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + Z::SMEM_ML / 4);
   uint64_t *k_full = bars, *k_empty = k_full + NS * DK, *v_full = k_empty + NS * DK, *v_empty = v_full + NS * DV, *s_full = v_empty + NS * DV;
   uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + NS, *raw_full = drain + NS;
   uint64_t *raw_empty = raw_full + 2 * Z::RAW, *sc_full = raw_empty + 2 * Z::RAW;  // K's, then V's
@@ -350,13 +358,13 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     }
     for (int i = 0; i < NB; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 8);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&drain[i], 1);
-      mbar_init(&q_full[i], 4 * NS);
+      mbar_init(&q_full[i], Z::SW);
     }
     for (int i = 0; i < 2 * Z::RAW; ++i) {
       mbar_init(&raw_full[i], 1);
@@ -375,7 +383,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   const TreeLine line = tree_line(a, pre);
   const int cta = blockIdx.x;
   if (cta >= line.ctas) return;
-  if (warp == 4 * NS + 2) {
+  if (warp == Z::SW + 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_s)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -390,14 +398,16 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   w.begun = false;
   uint32_t issued[2] = {0, 0};  // copies that a producer has requested, by ring
 
-  if (warp < 4 * NS) {
-    // ------------------------------------------------------------------ softmax: a thread has a row
-    const int st = warp >> 2, lg = warp & 3, row = lg * 32 + lane;
+  if (warp < Z::SW) {
+    // ------------------------------------------------------------------ softmax: a thread has a row's half of the tile
+    const int st = warp >> 3, hf = (warp >> 2) & 1, lg = warp & 3, row = lg * 32 + lane, who = 2 * st + hf;
+    const int pair_bar = 2 + 4 * st + lg;  // of the two warps that share rows
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(lg * 32) << 16);
     const uint32_t s_base = lane_base + st * 2 * KT, o_addr = lane_base + Z::O_COL + st * HD;
     const float c = fabsf(a.scale_log2);
     uint32_t uses[2] = {0, 0};  // of the stream's two S buffers
     uint32_t n_o = 0;           // segments in which the stream had a tile
+    uint32_t n_x = 0;           // exchanges of maxima with the other warp
     while (tm_next_segment(a, line, pre, w)) {
       const TreeSeg& sg = w.sg;
       const TreeSeq& sq = w.sq;
@@ -406,24 +416,25 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       const bool mine = row < rows;
       const bool used = mine && tok < sq.cnt;
       const unsigned long long bits = used ? tree_bits(a, sq, sg.b, tok) : 0ull;
+      const uint32_t cut = used ? 0xffffffffu : 0u;
       const bool warp_used = __any_sync(0xffffffffu, used);
       const int nt = sg.t1 - sg.t0;
-      // ---- Q: each of the NS warps of a lane group brings a part of the rows' boxes
+      // ---- Q: the 2 NS threads of a row bring its pieces
       {
         const T* src = static_cast<const T*>(a.q) + sg.b * a.q_seq + tok * a.q_tok + head * a.q_head;
         const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale goes with Q
-        constexpr int MINE = HD / 8 / NS, BATCH = MINE < 8 ? MINE : 8;  // 16-byte pieces of a row, requested together
+        constexpr int MINE = HD / 8 / (2 * NS), BATCH = MINE < 4 ? MINE : 4;  // 16-byte pieces of a row, requested together
 #pragma unroll 1
         for (int c0 = 0; c0 < MINE; c0 += BATCH) {
           uint4 v[BATCH];
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
-            const int ch = (c0 + i) * NS + st;
+            const int ch = (c0 + i) * 2 * NS + who;
             v[i] = used && ch * 8 < a.hd ? tm_load8(src + ch * 8, vec) : make_uint4(0, 0, 0, 0);  // hd is a multiple of 8
           }
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
-            const int ch = (c0 + i) * NS + st;
+            const int ch = (c0 + i) * 2 * NS + who;
             const uint4 f = make_uint4(v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
             *reinterpret_cast<uint4*>(q_t + (ch >> 3) * Z::QBOX + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = f;
           }
@@ -442,7 +453,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         const uint32_t n = uses[0] + uses[1];  // tiles of this stream before this one
         const uint32_t s_addr = s_base + buf * KT;
         const uint32_t ss = Z::CODED ? st * Z::SCALES + n % Z::SCALES : 0;
-        const float* sc = sc_s + ss * 3 * KT;
+        const float* sc = sc_s + ss * 3 * KT + 32 * hf;
         const uint32_t use = buf ? uses[1]++ : uses[0]++;
         bool ok = tm_wait(&s_full[2 * st + buf], use & 1, dead);
         if (Z::CODED) ok = tm_wait(&sc_full[ss], (n / Z::SCALES) & 1, dead) && ok;
@@ -451,12 +462,12 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           // does not see the node (those that do get it back at the end)
           if (DV < 2 && i >= NS) ok = tm_wait(&pv_done[st], (n - 1) & 1, dead) && ok;  // else the slot's phase before may still be open
           ok = tm_wait(&v_full[st * DV + n % DV], (n / DV) & 1, dead) && ok;
-          const int r = tid & 127, slot = s0 + r;
-          if (ok && r < KT && slot >= sq.len) {
+          const int r = tid & (KT - 1), part = (tid & 255) / KT, slot = s0 + r;  // four threads a row
+          if (ok && slot >= sq.len) {
             unsigned char* vr = v_t + (st * DV + n % DV) * Z::TILE + r * 128;
             bool bad = false;
 #pragma unroll 1
-            for (int ch = 0; ch < HD / 8; ++ch) {
+            for (int ch = part; ch < HD / 8; ch += 4) {
               uint4* at = reinterpret_cast<uint4*>(vr + (ch >> 3) * Z::BOX + (((ch + lane) & 7) << 4));
               if (slot >= sq.keys) {
                 *at = make_uint4(0, 0, 0, 0);
@@ -475,34 +486,45 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           }
         }
         ok = __all_sync(0xffffffffu, ok);
-        if (ok && warp_used) {
-          tm_fence_after();
-          uint32_t r[64];
-          tm_ld64(s_addr, r);
-          const uint32_t cut = used ? 0xffffffffu : 0u;
-          float mx = tail ? tm_row_max<STORE, true>(r, sc, s0, sq.len, bits, cut) : tm_row_max<STORE, false>(r, sc, s0, sq.len, bits, cut);
-          if (!Z::CODED && mx != -INFINITY) mx *= c;
-          if (__any_sync(0xffffffffu, mx > m + TM_SLACK)) {
+        if (warp_used) {  // both warps of the rows say the same here; what they do together depends on nothing that only one of them knows
+          uint32_t r[32];
+          float mx = -INFINITY;
+          if (ok) {
+            tm_fence_after();
+            tm_ld(s_addr + 32 * hf, r);
+            mx = tail ? tm_row_max<STORE, KT, true>(r, sc, s0 + 32 * hf, sq.len, bits, cut) : tm_row_max<STORE, KT, false>(r, sc, s0 + 32 * hf, sq.len, bits, cut);
+            if (!Z::CODED && mx != -INFINITY) mx *= c;
+            tm_fence_before();
+          }
+          // The first half's P lies over the first half's S, and so does the second half's: both S are read now.
+          if (tm_any64(pair_bar, mx > m + TM_SLACK)) {
+            float* mx_s = ml_s + (n_x++ & 1) * 2 * NS * TM_ROWS;
+            mx_s[who * TM_ROWS + row] = mx;
+            tm_any64(pair_bar, false);
+            mx = fmaxf(mx, mx_s[(who ^ 1) * TM_ROWS + row]);
             const float up = mx > m + TM_SLACK ? mx : m;
             const float f = up == m ? 1.f : exp2f(m - up);
             m = up;
             l *= f;
             if (i >= NS) {  // O holds something: the stream's last product has to be in it
               // Phase by parity: the one before it is over since S of this tile was formed, the one behind it waits for this tile's P.
-              ok = __all_sync(0xffffffffu, tm_wait(&pv_done[st], (n - 1) & 1, dead));
+              ok = __all_sync(0xffffffffu, tm_wait(&pv_done[st], (n - 1) & 1, dead)) && ok;
               tm_fence_after();
 #pragma unroll 1
-              for (int c0 = 0; c0 < HD; c0 += 16) {
+              for (int c0 = hf * (HD / 2); c0 < (hf + 1) * (HD / 2); c0 += 16) {
                 uint32_t o[16];
-                tm_ld16(o_addr + c0, o);
+                tm_ld(o_addr + c0, o);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
                 tm_st16(o_addr + c0, o);
               }
             }
           }
-          const float base = m == -INFINITY ? 0.f : m;
-          l += tail ? tm_row_weights<T, STORE, true>(r, s_addr, sc, c, base) : tm_row_weights<T, STORE, false>(r, s_addr, sc, c, base);
+          if (ok) {
+            tm_fence_after();
+            const float base = m == -INFINITY ? 0.f : m;
+            l += tail ? tm_row_weights<T, STORE, KT, true>(r, s_addr + 16 * hf, sc, c, base) : tm_row_weights<T, STORE, KT, false>(r, s_addr + 16 * hf, sc, c, base);
+          }
           tm_st_wait();
           tm_fence_before();
         }
@@ -519,107 +541,89 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         m = -INFINITY;
         l = 0.f;
       }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");  // bad_s of all warps; every product of the segment is done, every maximum read
+      ml_s[who * TM_ROWS + row] = m;
+      ml_s[(4 * NS + who) * TM_ROWS + row] = l;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
       float f = 1.f, big = m;
       if (NS == 2) {
-        ml_s[st * 2 * TM_ROWS + row] = m;
-        ml_s[(st * 2 + 1) * TM_ROWS + row] = l;
-      }
-      __syncwarp();
-      asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");  // m, l and bad_s of all warps; every product of the segment is done
-      if (NS == 2) {
-        const float mo = ml_s[(st ^ 1) * 2 * TM_ROWS + row], lo = ml_s[((st ^ 1) * 2 + 1) * TM_ROWS + row];
+        const float mo = ml_s[(who ^ 2) * TM_ROWS + row];
         big = fmaxf(m, mo);
         f = m == big ? 1.f : exp2f(m - big);
-        const float fo = mo == big ? 1.f : exp2f(mo - big);
-        l = l * f + lo * fo;
+      }
+      l = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * NS; ++k) {  // in the same order in every thread
+        const float mk = ml_s[k * TM_ROWS + row];
+        l += ml_s[(4 * NS + k) * TM_ROWS + row] * (mk == big ? 1.f : exp2f(mk - big));
       }
       const bool gone = !ok || *dead;
       const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
       const int slot = 2 * cta + (w.x == begin ? 0 : 1);
       float* po = tree_part_o(a, TM_ROWS, slot);
-      float* xch = reinterpret_cast<float*>(q_t);  // [columns][rows]: no product reads Q any more
+      float* xch = reinterpret_cast<float*>(q_t);  // [threads of a row][columns][rows]: no product reads Q any more
       const unsigned long long bad = bad_s & bits;
       T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + tok * a.o_tok + head * a.o_head;
       const float inv = big == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-      // Two streams: each finishes half of the columns, QW at a time, and hands the other its part of them.
-      constexpr int QW = NS == 2 ? HD / 4 : 16, ROUNDS = NS == 2 ? 2 : HD / 16;
+      // A row's threads finish a part of the columns each, QW at a time, and hand the thread of the other stream its part of them.
+      constexpr int COLS = HD / (2 * NS), QW = NS == 2 ? COLS / 2 : 16, ROUNDS = COLS / QW;
+      const int col0 = who * COLS;
 #pragma unroll 1
       for (int q = 0; q < ROUNDS; ++q) {
-        const int col = (NS == 2 ? st * (HD / 2) : 0) + q * QW;
-        if (NS == 2 && nt > 1) {
-          if (warp_used) {
-            const int give = (st ^ 1) * (HD / 2) + q * QW;
-            float* to = xch + st * (QW * TM_ROWS) + row;
+        const int col = col0 + q * QW;
+        if (NS == 2 && have && warp_used) {  // with one tile stream 1 has nothing to give
+          uint32_t r[QW];
+          tm_ld(o_addr + (who ^ 2) * COLS + q * QW, r);
 #pragma unroll
-            for (int c0 = 0; c0 < QW; c0 += 16) {
-              uint32_t r[16];
-              tm_ld16(o_addr + give + c0, r);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) to[(c0 + j) * TM_ROWS] = __uint_as_float(r[j]) * f;
-            }
-          }
-        } else if (NS == 2 && st == 0 && warp_used) {  // one tile: stream 1 has nothing, and its half comes from stream 0
-          float* to = xch + row;
-#pragma unroll
-          for (int c0 = 0; c0 < QW; c0 += 16) {
-            uint32_t r[16];
-            tm_ld16(o_addr + HD / 2 + q * QW + c0, r);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) to[(c0 + j) * TM_ROWS] = __uint_as_float(r[j]) * f;
-          }
+          for (int j = 0; j < QW; ++j) xch[(who * QW + j) * TM_ROWS + row] = __uint_as_float(r[j]) * f;
         }
         __syncwarp();
-        if (NS == 2) asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");
+        if (NS == 2) asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
         if (warp_used) {
-          const float* from = xch + (st ^ 1) * (QW * TM_ROWS) + row;
-#pragma unroll 1
-          for (int c0 = 0; c0 < QW; c0 += 16) {
-            float o[16];
-            if (have) {
-              uint32_t r[16];
-              tm_ld16(o_addr + col + c0, r);
+          float o[QW];
+          if (have) {
+            uint32_t r[QW];
+            tm_ld(o_addr + col, r);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __uint_as_float(r[j]) * f;
-            } else {
+            for (int j = 0; j < QW; ++j) o[j] = __uint_as_float(r[j]) * f;
+          } else {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = 0.f;
+            for (int j = 0; j < QW; ++j) o[j] = 0.f;
+          }
+          if (NS == 2 && (nt > 1 || st == 1)) {
+#pragma unroll
+            for (int j = 0; j < QW; ++j) o[j] += xch[((who ^ 2) * QW + j) * TM_ROWS + row];
+          }
+          // Nothing seen: what weights of zero met does not count.  A wait that expired: not a number.
+          if (gone || (big == -INFINITY && l == 0.f)) {
+#pragma unroll
+            for (int j = 0; j < QW; ++j) o[j] = gone ? __int_as_float(0x7fc00000) : 0.f;
+          }
+          if (whole) {
+            if (mine) {
+#pragma unroll
+              for (int j = 0; j < QW; j += 8)
+                if (col + j < a.hd)
+                  tm_store8(dst + col + j, vec,
+                            make_uint4(tm_pack<T>(o[j] * inv, o[j + 1] * inv), tm_pack<T>(o[j + 2] * inv, o[j + 3] * inv),
+                                       tm_pack<T>(o[j + 4] * inv, o[j + 5] * inv), tm_pack<T>(o[j + 6] * inv, o[j + 7] * inv)));
             }
-            if (NS == 2 && (nt > 1 || st == 1)) {
+          } else {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] += from[(c0 + j) * TM_ROWS];
-            }
-            // Nothing seen: what weights of zero met does not count.  A wait that expired: not a number.
-            if (gone || (big == -INFINITY && l == 0.f)) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = gone ? __int_as_float(0x7fc00000) : 0.f;
-            }
-            if (whole) {
-              if (mine) {
-#pragma unroll
-                for (int j = 0; j < 16; j += 8)
-                  if (col + c0 + j < a.hd)
-                    tm_store8(dst + col + c0 + j, vec,
-                              make_uint4(tm_pack<T>(o[j] * inv, o[j + 1] * inv), tm_pack<T>(o[j + 2] * inv, o[j + 3] * inv),
-                                         tm_pack<T>(o[j + 4] * inv, o[j + 5] * inv), tm_pack<T>(o[j + 6] * inv, o[j + 7] * inv)));
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; j += 4)
-                if (col + c0 + j < a.hd)
-                  *reinterpret_cast<float4*>(po + (static_cast<size_t>((col + c0 + j) / 4) * TM_ROWS + row) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            }
-            __syncwarp();
+            for (int j = 0; j < QW; j += 4)
+              if (col + j < a.hd)
+                *reinterpret_cast<float4*>(po + (static_cast<size_t>((col + j) / 4) * TM_ROWS + row) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
         } else if (whole && mine) {  // a warp of rows that are not in use: zeros
           for (int j = col; j < min(a.hd, col + QW); ++j) dst[j] = DT<T>::from_f(0.f);
         }
         __syncwarp();
-        if (NS == 2) asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");
+        if (NS == 2 && q + 1 < ROUNDS) asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
       }
       if (bad && !gone) {  // values that are not finite, for the rows that see them
         for (unsigned long long left = bad; left; left &= left - 1) {
           const auto* vr = vc.row(sg.b, sg.head, sq.len + __ffsll(static_cast<long long>(left)) - 1);
-          for (int d = st * (HD / 2); d < min(a.hd, NS == 2 ? (st + 1) * (HD / 2) : HD); ++d) {  // the columns that this thread has written
+          for (int d = col0; d < min(a.hd, col0 + COLS); ++d) {  // the columns that this thread has written
             const float v = held_value<T, STORE>(vr[d], 1.f);
             if (isfinite(v)) continue;
             if (whole) dst[d] = DT<T>::from_f(DT<T>::to_f(dst[d]) + v);
@@ -627,20 +631,19 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           }
         }
       }
-      __syncwarp();
-      if (st == 0 && !whole) {
+      if (who == 0 && !whole) {
         float* ml = tree_part_ml(a, TM_ROWS, slot);
         ml[row] = big;
         ml[TM_ROWS + row] = l;
       }
       tm_fence_before();
       __syncwarp();
-      asm volatile("bar.sync 1, %0;" ::"n"(128 * NS) : "memory");  // Q and bad_s are free
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");  // Q, m, l and bad_s are free
       if (tid == 0) bad_s = 0;
     }
-  } else if (warp < 4 * NS + 2) {
+  } else if (warp < Z::SW + 2) {
     // ------------------------------------------------------------------ TMA producers: one for K, one for V (a warp issues a box in about 150 ns)
-    const int half = warp - 4 * NS;
+    const int half = warp - Z::SW;
     const CUtensorMap* map = half ? &maps.v : &maps.k;
     constexpr uint32_t BYTES = Z::CODED ? Z::RAW_TILE : Z::TILE;
     const uint32_t d = Z::CODED ? Z::RAW : half ? DV : DK;
@@ -665,14 +668,14 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         issued[0] = n[0], issued[1] = n[1];
       }
     }
-  } else if (warp < 4 * NS + 2 + Z::ISSUERS) {
+  } else if (warp < Z::SW + 2 + Z::ISSUERS) {
     // ------------------------------------------------------------------ a stream's products
     {
       constexpr uint32_t fmt = DT<T>::id == STX_BF16 ? 1u : 0u;
       constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(TM_ROWS >> 4) << 24);
       constexpr uint32_t idesc_s = common | (static_cast<uint32_t>(KT >> 3) << 17);
       constexpr uint32_t idesc_o = common | (1u << 16) | (static_cast<uint32_t>(HD >> 3) << 17);  // V is MN-major
-      const int st = warp - (4 * NS + 2);
+      const int st = warp - (Z::SW + 2);
       uint32_t segs = 0, taken[2] = {0, 0};  // segments with a tile of the stream; uses of the stream's two P buffers
       uint32_t ns = 0, np = 0;               // S and P V of the stream so far
       bool ok = true;
@@ -725,7 +728,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     }
   } else if constexpr (Z::CODED) {
     // ------------------------------------------------------------------ codes become operands: two warps for K (and the scales), two for V
-    const int half = (warp - (4 * NS + 2 + Z::ISSUERS)) >> 1, ct = (tid & 31) + 32 * ((warp - (4 * NS + 2 + Z::ISSUERS)) & 1);
+    const int half = (warp - (Z::SW + 2 + Z::ISSUERS)) >> 1, ct = (tid & 31) + 32 * ((warp - (Z::SW + 2 + Z::ISSUERS)) & 1);
     const uint32_t d = half ? DV : DK;
     uint64_t *full = half ? v_full : k_full, *empty = half ? v_empty : k_empty;
     uint64_t *r_full = raw_full + half * Z::RAW, *r_empty = raw_empty + half * Z::RAW;
@@ -814,22 +817,22 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   tm_fence_before();
   __syncthreads();
   if (*dead) {  // a wait has expired: no copy and no product may still be on its way when the CTA leaves
-    if (warp >= 4 * NS && warp < 4 * NS + 2) {
-      const int half = warp - 4 * NS;
+    if (warp >= Z::SW && warp < Z::SW + 2) {
+      const int half = warp - Z::SW;
       const uint32_t d = Z::CODED ? Z::RAW : half ? DV : DK;
       uint64_t* full = Z::CODED ? raw_full + half * Z::RAW : half ? v_full : k_full;
       for (uint32_t st = 0; st < 2; ++st)
         for (uint32_t i = 0; i < d; ++i)
           if (issued[st] > i) mbar_wait_bounded(&full[st * d + i], ((issued[st] - 1 - i) / d) & 1);
-    } else if (warp >= 4 * NS + 2 && warp < 4 * NS + 2 + Z::ISSUERS) {
-      const int st = warp - (4 * NS + 2);
+    } else if (warp >= Z::SW + 2 && warp < Z::SW + 2 + Z::ISSUERS) {
+      const int st = warp - (Z::SW + 2);
       if (tm_elect()) tm_commit(&drain[st]);
       __syncwarp();
       mbar_wait_bounded(&drain[st], 0);
     }
     __syncthreads();
   }
-  if (warp == 4 * NS + 2) {
+  if (warp == Z::SW + 2) {
     tm_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
