@@ -34,7 +34,7 @@ constexpr int TM_ROWS = 128;
 constexpr float TM_SLACK = 8.f;  // in powers of two
 constexpr uint32_t TM_WAIT_LIMIT = 1u << 17;  // polls of up to 4 us: half a second
 
-template <int STORE, int HD> struct TmShape {
+template <int STORE, int HD, int REP> struct TmShape {
   static constexpr bool CODED = STORE != STX_STORE_SAME;
   static constexpr int KT = 64;                     // slots of a tile
   static constexpr int NS = HD == 256 ? 1 : 2;      // streams: two O of 256 columns do not fit next to S
@@ -45,24 +45,27 @@ template <int STORE, int HD> struct TmShape {
   static constexpr uint32_t QBOX = TM_ROWS * 128, Q = BOXES * QBOX;
   // Tiles in shared memory (16-bit), in a ring for each stream: whoever waits for a slot then knows its ring's earlier phases to be over, and
   // a phase's parity is not taken for another's.  What an SM has to have on its way is 45 KB (0.3 KB/ns of HBM x 148 SMs at 1 us).
-  static constexpr int DK = HD == 64 ? (CODED ? 3 : 4) : HD == 128 ? (CODED ? 2 : 3) : 2;
-  static constexpr int DV = HD == 64 ? (CODED ? 2 : 3) : HD == 128 ? 2 : CODED ? 1 : 2;
+  static constexpr int DK = HD == 64 ? (CODED ? 3 : 4) : 2;
+  static constexpr int DV = HD == 64 ? (CODED ? 2 : 4) : HD == 128 ? (CODED ? 2 : 3) : CODED ? 1 : 2;
   static constexpr int RAW = CODED ? (HD == 64 ? 6 : HD == 128 ? 3 : 1) : 0;  // tiles of codes of K, and as many of V
   static constexpr uint32_t RAW_TILE = KT * HD;
   // Tiles of a stream whose scales are kept: those of tile c are overwritten with K of tile c + SCALES, which waits for S of tile c + 2, formed
   // in the place of P of tile c.
   static constexpr int SCALES = DK + 2;
   static constexpr int ISSUERS = NS;                // warps that issue products, one for each stream
-  static constexpr int SW = 8 * NS;                  // warps of the soft-max: a lane group's rows x two halves of the tile, for each stream
-  static constexpr int WARPS = SW + 2 + ISSUERS + (CODED ? 4 : 0);
+  static constexpr int HF = REP == 1 ? 2 : 1;       // threads that share a row's part of a tile
+  static constexpr int SW = 4 * HF * NS;            // warps of the soft-max
+  static constexpr int CONV = CODED ? 8 : 0;        // warps that convert, half of them K
+  static constexpr int WARPS = SW + 2 + ISSUERS + CONV;
   static constexpr int THREADS = 32 * WARPS;
   static constexpr uint32_t O_COL = 256;
-  static constexpr uint32_t SMEM_TILES = Q + NS * (DK + DV) * TILE + 2 * RAW * RAW_TILE;
+  static constexpr uint32_t QX = Q < 32768 ? 32768 : Q;  // Q, later the exchange of a segment's end
+  static constexpr uint32_t SMEM_TILES = QX + NS * (DK + DV) * TILE + 2 * RAW * RAW_TILE;
   static constexpr uint32_t SMEM_SCALES = CODED ? NS * SCALES * 3 * KT * 4 : 0;
-  static constexpr uint32_t SMEM_ML = 3 * 2 * NS * TM_ROWS * 4;  // m (of tile and segment) and l of each thread of the soft-max
+  static constexpr uint32_t SMEM_ML = 3 * HF * NS * TM_ROWS * 4;  // m (of tile and segment) and l of each thread of the soft-max
   static constexpr uint32_t BARS = 2 * NS * (DK + DV) + 2 * NB + 4 * NS + 4 * RAW + (CODED ? NS * SCALES : 0);
   static constexpr uint32_t SMEM = 1024 + SMEM_TILES + SMEM_SCALES + SMEM_ML + BARS * 8 + 64;
-  static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1) + 64 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1 + TM_ROWS) + 64 <= 227 * 1024, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
@@ -118,15 +121,6 @@ __device__ __forceinline__ void tm_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 }
 // Columns of the warp's 32 lanes.  The wait is part of the statement: between the two the compiler could move registers that are not
 // there yet (it does where it has to spill).
-__device__ __forceinline__ void tm_ld(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-      : "r"(taddr)
-      : "memory");
-}
 __device__ __forceinline__ void tm_ld(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -150,7 +144,12 @@ __device__ __forceinline__ void tm_ld(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tm_st(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+               "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tm_st(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
@@ -187,16 +186,39 @@ __device__ __forceinline__ uint4 tm_load8(const T* p, int vec) {
                     u[6] | static_cast<uint32_t>(u[7]) << 16);
 }
 
-template <typename T>
-__device__ __forceinline__ void tm_store8(T* p, int vec, const uint4& v) {
-  if (vec) {
-    st16(p, v);
-    return;
-  }
-  unsigned short* u = reinterpret_cast<unsigned short*>(p);
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// N values of a row (N: 2, 4, 8 or 16), `left` of them inside the head.
+template <typename T, int N>
+__device__ __forceinline__ void tm_store(T* p, int vec, const float (&o)[N], int left) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)));
+  for (int j = 0; j < N; j += 8) {
+    if (j >= left) break;
+    constexpr int M = N < 8 ? N : 8;
+    uint32_t w[M / 2];
+#pragma unroll
+    for (int i = 0; i < M / 2; ++i) w[i] = tm_pack<T>(o[j + 2 * i], o[j + 2 * i + 1]);
+    if (vec) {
+      if constexpr (M == 8) st16(p + j, make_uint4(w[0], w[1], w[2], w[3]));
+      else if constexpr (M == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(p) = w[0];
+    } else {
+      unsigned short* u = reinterpret_cast<unsigned short*>(p + j);
+#pragma unroll
+      for (int i = 0; i < M; ++i) u[i] = static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+// Adds the values of the nodes in `nodes` that are not finite (they were left out of the products) to n results that this thread has just
+// written: a row's values (rows 1, p at column `col`), or fp32 values four columns apart by `rows` (p at column 0).
+template <typename T, int STORE, typename P>
+__device__ __noinline__ void tm_add_bad(P* p, int rows, unsigned long long nodes, KvPtr<typename Held<T, STORE>::C> vc, int b, int head, int len, int col, int n) {
+  for (; nodes; nodes &= nodes - 1) {
+    const auto* vr = vc.row(b, head, len + __ffsll(static_cast<long long>(nodes)) - 1) + col;
+    for (int j = 0; j < n; ++j) {
+      const float v = held_value<T, STORE>(vr[j], 1.f);
+      P* at = rows == 1 ? p + j : p + static_cast<size_t>((col + j) / 4) * rows * 4 + (col + j) % 4;
+      if (!isfinite(v)) *at = DT<P>::from_f(DT<P>::to_f(*at) + v);
+    }
+  }
 }
 
 // Two 16-bit operands from two codes.  int8: the byte is put under the exponent of a number whose last place is 1, and that number
@@ -262,14 +284,14 @@ __device__ __forceinline__ void tm_load(void* dst, const CUtensorMap* m, int ord
       : "memory");
 }
 
-// x of 32 slots from their S (16-bit caches: S itself), what the row does not see as -infinity, and the largest of them.  TAIL: there are
+// x of N slots from their S (16-bit caches: S itself), what the row does not see as -infinity, and the largest of them.  TAIL: there are
 // slots that the row may not see; `cut` is 0 for rows that are not in use.  The two forms are apart so that the common one has no masks in it.
-template <int STORE, int KT, bool TAIL>
-__device__ __forceinline__ float tm_row_max(uint32_t (&r)[32], const float* sc, int s0, int len, unsigned long long bits, uint32_t cut) {
+template <int STORE, int KT, bool TAIL, int N>
+__device__ __forceinline__ float tm_row_max(uint32_t (&r)[N], const float* sc, int s0, int len, unsigned long long bits, uint32_t cut) {
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   const uint32_t v = TAIL ? tree_visible(s0, len, bits) & cut : ~0u;
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     float x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(r[j + e]);
@@ -286,13 +308,13 @@ __device__ __forceinline__ float tm_row_max(uint32_t (&r)[32], const float* sc, 
   }
   return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
-// P = 2^(x - base), packed in pairs, to 16 columns from p_addr on; returns the sum of the weights.
-template <typename T, int STORE, int KT, bool TAIL>
-__device__ __forceinline__ float tm_row_weights(const uint32_t (&r)[32], uint32_t p_addr, const float* sc, float c, float base) {
+// P = 2^(x - base), packed in pairs, to N / 2 columns from p_addr on; returns the sum of the weights.
+template <typename T, int STORE, int KT, bool TAIL, int N>
+__device__ __forceinline__ float tm_row_weights(const uint32_t (&r)[N], uint32_t p_addr, const float* sc, float c, float base) {
   float l[4] = {0.f, 0.f, 0.f, 0.f};
-  uint32_t p16[16];
+  uint32_t p16[N / 2];
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     float p[4], iv[4] = {1.f, 1.f, 1.f, 1.f};
     if constexpr (STORE != STX_STORE_SAME) {
       const float4 ii = *reinterpret_cast<const float4*>(sc + 2 * KT + j);
@@ -308,7 +330,7 @@ __device__ __forceinline__ float tm_row_weights(const uint32_t (&r)[32], uint32_
     p16[j / 2] = tm_pack<T>(p[0], p[1]);
     p16[j / 2 + 1] = tm_pack<T>(p[2], p[3]);
   }
-  tm_st16(p_addr, p16);
+  tm_st(p_addr, p16);
   return (l[0] + l[1]) + (l[2] + l[3]);
 }
 // Whether any of the 64 threads of two warps says so; also a barrier of theirs.
@@ -322,24 +344,25 @@ __device__ __forceinline__ bool tm_any64(int bar, bool mine) {
   return r != 0;
 }
 
-template <typename T, int STORE, int HD>
-__global__ void __launch_bounds__(TmShape<STORE, HD>::THREADS, 1)
+template <typename T, int STORE, int HD, int REP>
+__global__ void __launch_bounds__(TmShape<STORE, HD, REP>::THREADS, 1)
 k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvPtr<typename Held<T, STORE>::C> kc,
                 const KvPtr<typename Held<T, STORE>::C> vc, int vec) {
-  typedef TmShape<STORE, HD> Z;
-  constexpr int KT = Z::KT, NS = Z::NS, NB = Z::NB, DK = Z::DK, DV = Z::DV;
+  typedef TmShape<STORE, HD, REP> Z;
+  constexpr int KT = Z::KT, NS = Z::NS, HF = Z::HF, NB = Z::NB, DK = Z::DK, DV = Z::DV;
   extern __shared__ unsigned char tm_raw[];
   __shared__ int pre[TREE_MAX_SEQ + 1];
   __shared__ unsigned long long bad_s;  // nodes of the segment with a value that is not finite
   __shared__ uint32_t tmem_s;
+  __shared__ float inv_s[TM_ROWS];
   __shared__ int dead_s;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* q_t = smem;
-  unsigned char* k_t = q_t + Z::Q;
+  unsigned char* k_t = q_t + Z::QX;
   unsigned char* v_t = k_t + NS * DK * Z::TILE;
   unsigned char* raw_t = v_t + NS * DV * Z::TILE;
   float* sc_s = reinterpret_cast<float*>(raw_t + 2 * Z::RAW * Z::RAW_TILE);  // [SCALES][3][KT]
-  float* ml_s = sc_s + Z::SMEM_SCALES / 4;  // m of a tile, two in turn [2][2 NS][TM_ROWS] (the first also: m of a segment), l [2 NS][TM_ROWS]
+  float* ml_s = sc_s + Z::SMEM_SCALES / 4;  // m of a tile, two in turn [2][HF NS][TM_ROWS] (the first also: m of a segment), l [HF NS][TM_ROWS]
   uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + Z::SMEM_ML / 4);
   uint64_t *k_full = bars, *k_empty = k_full + NS * DK, *v_full = k_empty + NS * DK, *v_empty = v_full + NS * DV, *s_full = v_empty + NS * DV;
   uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + NS, *raw_full = drain + NS;
@@ -349,16 +372,16 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
 
   if (tid == 0) {
     for (int i = 0; i < NS * DK; ++i) {
-      mbar_init(&k_full[i], Z::CODED ? 2 : 1);
+      mbar_init(&k_full[i], Z::CODED ? Z::CONV / 2 : 1);
       mbar_init(&k_empty[i], 1);
     }
     for (int i = 0; i < NS * DV; ++i) {
-      mbar_init(&v_full[i], Z::CODED ? 2 : 1);
+      mbar_init(&v_full[i], Z::CODED ? Z::CONV / 2 : 1);
       mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < NB; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
+      mbar_init(&p_full[i], 4 * HF);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&pv_done[i], 1);
@@ -368,7 +391,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     }
     for (int i = 0; i < 2 * Z::RAW; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 2);
+      mbar_init(&raw_empty[i], Z::CONV / 2);
     }
     if (Z::CODED)
       for (int i = 0; i < NS * Z::SCALES; ++i) mbar_init(&sc_full[i], 2);
@@ -400,8 +423,12 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
 
   if (warp < Z::SW) {
     // ------------------------------------------------------------------ softmax: a thread has a row's half of the tile
-    const int st = warp >> 3, hf = (warp >> 2) & 1, lg = warp & 3, row = lg * 32 + lane, who = 2 * st + hf;
-    const int pair_bar = 2 + 4 * st + lg;  // of the two warps that share rows
+    // REP = 4 (up to 32 rows): the rows stand in all four lane groups, and each group takes a quarter of a tile's slots, with m, l and O of its
+    // own that are added at the end: as the powers of a warp's lanes cost the same however few of them are in use, this is a quarter of the work.
+    constexpr int RR = TM_ROWS / REP, CW = KT / REP / HF;  // rows; slots of a thread
+    const int st = warp / (4 * HF), hf = (warp >> 2) % HF, lg = warp & 3, tl = lg * 32 + lane, who = HF * st + hf;
+    const int row = tl % RR, rep = tl / RR, cs = rep * (KT / REP) + hf * CW;  // cs: the first slot of this thread
+    const int pair_bar = 2 + 4 * st + lg;  // of two warps that share rows
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(lg * 32) << 16);
     const uint32_t s_base = lane_base + st * 2 * KT, o_addr = lane_base + Z::O_COL + st * HD;
     const float c = fabsf(a.scale_log2);
@@ -419,24 +446,24 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       const uint32_t cut = used ? 0xffffffffu : 0u;
       const bool warp_used = __any_sync(0xffffffffu, used);
       const int nt = sg.t1 - sg.t0;
-      // ---- Q: the 2 NS threads of a row bring its pieces
+      // ---- Q: a row's threads bring its pieces
       {
         const T* src = static_cast<const T*>(a.q) + sg.b * a.q_seq + tok * a.q_tok + head * a.q_head;
         const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale goes with Q
-        constexpr int MINE = HD / 8 / (2 * NS), BATCH = MINE < 4 ? MINE : 4;  // 16-byte pieces of a row, requested together
+        constexpr int MINE = HD / 8 / (HF * NS), BATCH = MINE < 4 ? MINE : 4;  // 16-byte pieces of a row, requested together
 #pragma unroll 1
         for (int c0 = 0; c0 < MINE; c0 += BATCH) {
           uint4 v[BATCH];
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
-            const int ch = (c0 + i) * 2 * NS + who;
+            const int ch = (c0 + i) * HF * NS + who;
             v[i] = used && ch * 8 < a.hd ? tm_load8(src + ch * 8, vec) : make_uint4(0, 0, 0, 0);  // hd is a multiple of 8
           }
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
-            const int ch = (c0 + i) * 2 * NS + who;
+            const int ch = (c0 + i) * HF * NS + who;
             const uint4 f = make_uint4(v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
-            *reinterpret_cast<uint4*>(q_t + (ch >> 3) * Z::QBOX + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = f;
+            *reinterpret_cast<uint4*>(q_t + (ch >> 3) * Z::QBOX + tl * 128 + (((ch & 7) ^ (tl & 7)) << 4)) = f;
           }
         }
         tm_fence_async();
@@ -453,7 +480,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         const uint32_t n = uses[0] + uses[1];  // tiles of this stream before this one
         const uint32_t s_addr = s_base + buf * KT;
         const uint32_t ss = Z::CODED ? st * Z::SCALES + n % Z::SCALES : 0;
-        const float* sc = sc_s + ss * 3 * KT + 32 * hf;
+        const float* sc = sc_s + ss * 3 * KT + cs;
         const uint32_t use = buf ? uses[1]++ : uses[0]++;
         bool ok = tm_wait(&s_full[2 * st + buf], use & 1, dead);
         if (Z::CODED) ok = tm_wait(&sc_full[ss], (n / Z::SCALES) & 1, dead) && ok;
@@ -462,12 +489,12 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           // does not see the node (those that do get it back at the end)
           if (DV < 2 && i >= NS) ok = tm_wait(&pv_done[st], (n - 1) & 1, dead) && ok;  // else the slot's phase before may still be open
           ok = tm_wait(&v_full[st * DV + n % DV], (n / DV) & 1, dead) && ok;
-          const int r = tid & (KT - 1), part = (tid & 255) / KT, slot = s0 + r;  // four threads a row
+          const int r = tid & (KT - 1), part = (tid % (128 * HF)) / KT, slot = s0 + r;
           if (ok && slot >= sq.len) {
             unsigned char* vr = v_t + (st * DV + n % DV) * Z::TILE + r * 128;
             bool bad = false;
 #pragma unroll 1
-            for (int ch = part; ch < HD / 8; ch += 4) {
+            for (int ch = part; ch < HD / 8; ch += 2 * HF) {
               uint4* at = reinterpret_cast<uint4*>(vr + (ch >> 3) * Z::BOX + (((ch + lane) & 7) << 4));
               if (slot >= sq.keys) {
                 *at = make_uint4(0, 0, 0, 0);
@@ -487,21 +514,23 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         }
         ok = __all_sync(0xffffffffu, ok);
         if (warp_used) {  // both warps of the rows say the same here; what they do together depends on nothing that only one of them knows
-          uint32_t r[32];
+          uint32_t r[CW];
           float mx = -INFINITY;
           if (ok) {
             tm_fence_after();
-            tm_ld(s_addr + 32 * hf, r);
-            mx = tail ? tm_row_max<STORE, KT, true>(r, sc, s0 + 32 * hf, sq.len, bits, cut) : tm_row_max<STORE, KT, false>(r, sc, s0 + 32 * hf, sq.len, bits, cut);
+            tm_ld(s_addr + cs, r);
+            mx = tail ? tm_row_max<STORE, KT, true>(r, sc, s0 + cs, sq.len, bits, cut) : tm_row_max<STORE, KT, false>(r, sc, s0 + cs, sq.len, bits, cut);
             if (!Z::CODED && mx != -INFINITY) mx *= c;
             tm_fence_before();
           }
-          // The first half's P lies over the first half's S, and so does the second half's: both S are read now.
-          if (tm_any64(pair_bar, mx > m + TM_SLACK)) {
-            float* mx_s = ml_s + (n_x++ & 1) * 2 * NS * TM_ROWS;
-            mx_s[who * TM_ROWS + row] = mx;
-            tm_any64(pair_bar, false);
-            mx = fmaxf(mx, mx_s[(who ^ 1) * TM_ROWS + row]);
+          // P lies over the first half of S: two warps that share a row have read theirs now.
+          if (HF == 2 ? tm_any64(pair_bar, mx > m + TM_SLACK) : __any_sync(0xffffffffu, mx > m + TM_SLACK)) {
+            if (HF == 2) {
+              float* mx_s = ml_s + (n_x++ & 1) * HF * NS * TM_ROWS;
+              mx_s[who * TM_ROWS + tl] = mx;
+              tm_any64(pair_bar, false);
+              mx = fmaxf(mx, mx_s[(who ^ 1) * TM_ROWS + tl]);
+            }
             const float up = mx > m + TM_SLACK ? mx : m;
             const float f = up == m ? 1.f : exp2f(m - up);
             m = up;
@@ -511,19 +540,24 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
               ok = __all_sync(0xffffffffu, tm_wait(&pv_done[st], (n - 1) & 1, dead)) && ok;
               tm_fence_after();
 #pragma unroll 1
-              for (int c0 = hf * (HD / 2); c0 < (hf + 1) * (HD / 2); c0 += 16) {
+              for (int c0 = hf * (HD / HF); c0 < (hf + 1) * (HD / HF); c0 += 16) {
                 uint32_t o[16];
                 tm_ld(o_addr + c0, o);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                tm_st16(o_addr + c0, o);
+                tm_st(o_addr + c0, o);
               }
             }
           }
           if (ok) {
             tm_fence_after();
             const float base = m == -INFINITY ? 0.f : m;
-            l += tail ? tm_row_weights<T, STORE, KT, true>(r, s_addr + 16 * hf, sc, c, base) : tm_row_weights<T, STORE, KT, false>(r, s_addr + 16 * hf, sc, c, base);
+            l += tail ? tm_row_weights<T, STORE, KT, true>(r, s_addr + cs / 2, sc, c, base) : tm_row_weights<T, STORE, KT, false>(r, s_addr + cs / 2, sc, c, base);
+#pragma unroll
+            for (int k = 1; k < REP; ++k) {  // the slots of the other lane groups weigh nothing here
+              const uint32_t zero[CW / 2] = {};
+              tm_st(s_addr + ((rep + k) % REP) * (KT / REP / 2) + hf * (CW / 2), zero);
+            }
           }
           tm_st_wait();
           tm_fence_before();
@@ -542,99 +576,84 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         l = 0.f;
       }
       asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");  // bad_s of all warps; every product of the segment is done, every maximum read
-      ml_s[who * TM_ROWS + row] = m;
-      ml_s[(4 * NS + who) * TM_ROWS + row] = l;
+      ml_s[who * TM_ROWS + tl] = m;
+      ml_s[(2 * HF * NS + who) * TM_ROWS + tl] = l;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
-      float f = 1.f, big = m;
-      if (NS == 2) {
-        const float mo = ml_s[(who ^ 2) * TM_ROWS + row];
-        big = fmaxf(m, mo);
-        f = m == big ? 1.f : exp2f(m - big);
-      }
-      l = 0.f;
+      // The row's results, NS streams x REP lane groups: M, and each one's share of the sum, 2^(m - M), in the same order everywhere.
+      float big = m;
 #pragma unroll
-      for (int k = 0; k < 2 * NS; ++k) {  // in the same order in every thread
-        const float mk = ml_s[k * TM_ROWS + row];
-        l += ml_s[(4 * NS + k) * TM_ROWS + row] * (mk == big ? 1.f : exp2f(mk - big));
-      }
+      for (int k = 0; k < NS * REP; ++k) big = fmaxf(big, ml_s[HF * (k / REP) * TM_ROWS + (k % REP) * RR + row]);
+      const float f = m == big ? 1.f : exp2f(m - big);
       const bool gone = !ok || *dead;
       const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
       const int slot = 2 * cta + (w.x == begin ? 0 : 1);
       float* po = tree_part_o(a, TM_ROWS, slot);
-      float* xch = reinterpret_cast<float*>(q_t);  // [threads of a row][columns][rows]: no product reads Q any more
-      const unsigned long long bad = bad_s & bits;
-      T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + tok * a.o_tok + head * a.o_head;
-      const float inv = big == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-      // A row's threads finish a part of the columns each, QW at a time, and hand the thread of the other stream its part of them.
-      constexpr int COLS = HD / (2 * NS), QW = NS == 2 ? COLS / 2 : 16, ROUNDS = COLS / QW;
-      const int col0 = who * COLS;
-#pragma unroll 1
-      for (int q = 0; q < ROUNDS; ++q) {
-        const int col = col0 + q * QW;
-        if (NS == 2 && have && warp_used) {  // with one tile stream 1 has nothing to give
-          uint32_t r[QW];
-          tm_ld(o_addr + (who ^ 2) * COLS + q * QW, r);
+      if (who == 0 && rep == 0) {
+        float sum = 0.f;
 #pragma unroll
-          for (int j = 0; j < QW; ++j) xch[(who * QW + j) * TM_ROWS + row] = __uint_as_float(r[j]) * f;
+        for (int k = 0; k < NS * REP; ++k) {
+          const int at = HF * (k / REP) * TM_ROWS + (k % REP) * RR + row;
+          const float mk = ml_s[at];
+          float lk = ml_s[2 * HF * NS * TM_ROWS + at];
+          if (HF == 2) lk += ml_s[(2 * HF * NS + 1) * TM_ROWS + at];
+          sum += lk * (mk == big ? 1.f : exp2f(mk - big));
         }
-        __syncwarp();
-        if (NS == 2) asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
-        if (warp_used) {
-          float o[QW];
-          if (have) {
-            uint32_t r[QW];
-            tm_ld(o_addr + col, r);
+        // 1 / l; 0 where nothing was seen (what weights of zero met does not count), NaN where a wait has expired
+        inv_s[row] = gone ? __int_as_float(0x7fc00000) : big == -INFINITY && sum == 0.f ? 0.f : whole ? 1.f / sum : 1.f;
+        if (!whole) {
+          float* ml = tree_part_ml(a, TM_ROWS, slot);
+          ml[row] = big;
+          ml[TM_ROWS + row] = sum;
+        }
+      }
+      // C columns at a time: every thread brings its half of them, scaled, to shared memory (over Q, which no product reads any more),
+      // [stream and lane group][column][row], and takes EL columns of a row from there.
+      constexpr int C = 32, EL = RR * C / (32 * Z::SW);
+      float* xch = reinterpret_cast<float*>(q_t);
+      const int orow = tid % RR, ocol = tid / RR * EL;
+      const int otok = tok0 + orow / a.group;
+      const unsigned long long bad = bad_s;
+#pragma unroll 1
+      for (int c0 = 0; c0 < HD; c0 += C) {
+        {
+          float* to = xch + ((st * REP + rep) * C + hf * (C / HF)) * RR + row;
+          if (have && warp_used) {
+            uint32_t r[C / HF];
+            tm_ld(o_addr + c0 + hf * (C / HF), r);
 #pragma unroll
-            for (int j = 0; j < QW; ++j) o[j] = __uint_as_float(r[j]) * f;
+            for (int j = 0; j < C / HF; ++j) to[j * RR] = used ? __uint_as_float(r[j]) * f : 0.f;
           } else {
 #pragma unroll
-            for (int j = 0; j < QW; ++j) o[j] = 0.f;
+            for (int j = 0; j < C / HF; ++j) to[j * RR] = 0.f;
           }
-          if (NS == 2 && (nt > 1 || st == 1)) {
+        }
+        __syncwarp();
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
+        const int col = c0 + ocol;
+        if (orow < rows && col < a.hd) {  // hd is a multiple of 8, and EL divides 8 or is a multiple of it
+          float o[EL];
+          const float inv = inv_s[orow];
 #pragma unroll
-            for (int j = 0; j < QW; ++j) o[j] += xch[((who ^ 2) * QW + j) * TM_ROWS + row];
-          }
-          // Nothing seen: what weights of zero met does not count.  A wait that expired: not a number.
-          if (gone || (big == -INFINITY && l == 0.f)) {
+          for (int j = 0; j < EL; ++j) {
+            o[j] = 0.f;
 #pragma unroll
-            for (int j = 0; j < QW; ++j) o[j] = gone ? __int_as_float(0x7fc00000) : 0.f;
+            for (int k = 0; k < NS * REP; ++k) o[j] += xch[(k * C + ocol + j) * RR + orow];
+            o[j] = inv == 0.f ? 0.f : o[j] * inv;
           }
           if (whole) {
-            if (mine) {
-#pragma unroll
-              for (int j = 0; j < QW; j += 8)
-                if (col + j < a.hd)
-                  tm_store8(dst + col + j, vec,
-                            make_uint4(tm_pack<T>(o[j] * inv, o[j + 1] * inv), tm_pack<T>(o[j + 2] * inv, o[j + 3] * inv),
-                                       tm_pack<T>(o[j + 4] * inv, o[j + 5] * inv), tm_pack<T>(o[j + 6] * inv, o[j + 7] * inv)));
-            }
+            T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + otok * a.o_tok + (sg.head * a.group + orow % a.group) * a.o_head + col;
+            tm_store<T, EL>(dst, vec, o, a.hd - col);
+            if (bad) tm_add_bad<T, STORE>(dst, 1, bad & tree_bits(a, sq, sg.b, otok), vc, sg.b, sg.head, sq.len, col, min(EL, a.hd - col));
           } else {
 #pragma unroll
-            for (int j = 0; j < QW; j += 4)
+            for (int j = 0; j < EL; j += 2)
               if (col + j < a.hd)
-                *reinterpret_cast<float4*>(po + (static_cast<size_t>((col + j) / 4) * TM_ROWS + row) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                *reinterpret_cast<float2*>(po + (static_cast<size_t>((col + j) / 4) * TM_ROWS + orow) * 4 + (col + j) % 4) = make_float2(o[j], o[j + 1]);
+            if (bad) tm_add_bad<T, STORE>(po + static_cast<size_t>(orow) * 4, TM_ROWS, bad & tree_bits(a, sq, sg.b, otok), vc, sg.b, sg.head, sq.len, col, min(EL, a.hd - col));
           }
-        } else if (whole && mine) {  // a warp of rows that are not in use: zeros
-          for (int j = col; j < min(a.hd, col + QW); ++j) dst[j] = DT<T>::from_f(0.f);
         }
         __syncwarp();
-        if (NS == 2 && q + 1 < ROUNDS) asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
-      }
-      if (bad && !gone) {  // values that are not finite, for the rows that see them
-        for (unsigned long long left = bad; left; left &= left - 1) {
-          const auto* vr = vc.row(sg.b, sg.head, sq.len + __ffsll(static_cast<long long>(left)) - 1);
-          for (int d = col0; d < min(a.hd, col0 + COLS); ++d) {  // the columns that this thread has written
-            const float v = held_value<T, STORE>(vr[d], 1.f);
-            if (isfinite(v)) continue;
-            if (whole) dst[d] = DT<T>::from_f(DT<T>::to_f(dst[d]) + v);
-            else po[(static_cast<size_t>(d / 4) * TM_ROWS + row) * 4 + d % 4] += v;
-          }
-        }
-      }
-      if (who == 0 && !whole) {
-        float* ml = tree_part_ml(a, TM_ROWS, slot);
-        ml[row] = big;
-        ml[TM_ROWS + row] = l;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
       }
       tm_fence_before();
       __syncwarp();
@@ -727,8 +746,9 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       }
     }
   } else if constexpr (Z::CODED) {
-    // ------------------------------------------------------------------ codes become operands: two warps for K (and the scales), two for V
-    const int half = (warp - (Z::SW + 2 + Z::ISSUERS)) >> 1, ct = (tid & 31) + 32 * ((warp - (Z::SW + 2 + Z::ISSUERS)) & 1);
+    // ------------------------------------------------------------------ codes become operands: half of the warps for K (and the scales), half for V
+    constexpr int CT = 16 * Z::CONV;  // threads of a half
+    const int half = (tid - 32 * (Z::SW + 2 + Z::ISSUERS)) / CT, ct = (tid - 32 * (Z::SW + 2 + Z::ISSUERS)) % CT;
     const uint32_t d = half ? DV : DK;
     uint64_t *full = half ? v_full : k_full, *empty = half ? v_empty : k_empty;
     uint64_t *r_full = raw_full + half * Z::RAW, *r_empty = raw_empty + half * Z::RAW;
@@ -739,7 +759,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     bool ok = true;
     // the scales of a tile are requested a tile ahead
     TmWalk ahead = w;
-    bool more = half == 0 && tm_next_segment(a, line, pre, ahead);
+    bool more = half == 0 && ct < KT && tm_next_segment(a, line, pre, ahead);
     float ks = 0.f, vs = 0.f;
     auto request = [&]() {
       ks = 0.f;
@@ -761,17 +781,17 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         ok = ok && tm_wait(&r_full[rs], ruse & 1, dead);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        constexpr int PER = HD / 16, EACH = KT * PER / 64;  // 16-byte pieces of a row of codes, of a thread
+        constexpr int PER = HD / 16, EACH = KT * PER / CT, BATCH = EACH < 4 ? EACH : 4;  // 16-byte pieces of a row of codes, of a thread
         const unsigned char* src = raw + rs * Z::RAW_TILE;
         unsigned char* dst = tiles_t + s * Z::TILE;
 #pragma unroll
-        for (int i0 = 0; i0 < EACH; i0 += 4) {
-          uint4 w4[4];
+        for (int i0 = 0; i0 < EACH; i0 += BATCH) {
+          uint4 w4[BATCH];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w4[i] = *reinterpret_cast<const uint4*>(src + (ct + 64 * (i0 + i)) * 16);
+          for (int i = 0; i < BATCH; ++i) w4[i] = *reinterpret_cast<const uint4*>(src + (ct + CT * (i0 + i)) * 16);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = ct + 64 * (i0 + i), r = at / PER, piece = at % PER;
+          for (int i = 0; i < BATCH; ++i) {
+            const int at = ct + CT * (i0 + i), r = at / PER, piece = at % PER;
             const uint32_t q4[4] = {w4[i].x, w4[i].y, w4[i].z, w4[i].w};
             uint32_t e[8];
 #pragma unroll
@@ -795,7 +815,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           tm_arrive(&r_empty[rs]);
           tm_arrive(&full[s]);
         }
-        if (half == 0) {
+        if (half == 0 && ct < KT) {
           const float v = vs == 0.f ? 1.f : vs;  // a row of zeros: any scale
           const uint32_t ss = st * Z::SCALES + m % Z::SCALES;
           float* sc = sc_s + ss * 3 * KT;
@@ -903,9 +923,9 @@ static int tm_map(CUtensorMap* m, const void* base, const stx_kv* c, const TmOrd
   return STX_OK;
 }
 
-template <typename T, int STORE, int HD>
+template <typename T, int STORE, int HD, int REP>
 static int launch_mma(TreeArgs a, const stx_kv* cache, const TmOrder& o, int vec, cudaStream_t s) {
-  typedef TmShape<STORE, HD> Z;
+  typedef TmShape<STORE, HD, REP> Z;
   typedef typename Held<T, STORE>::C C;
   TmMaps maps;
   int rc = tm_map(&maps.k, cache->k, cache, o, Z::CODED ? HD : 64, Z::KT);
@@ -916,10 +936,10 @@ static int launch_mma(TreeArgs a, const stx_kv* cache, const TmOrder& o, int vec
   int dev = 0;
   STX_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    STX_CUDA(cudaFuncSetAttribute(k_tree_attn_mma<T, STORE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Z::SMEM)));
+    STX_CUDA(cudaFuncSetAttribute(k_tree_attn_mma<T, STORE, HD, REP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Z::SMEM)));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  STX_CUDA(launch_pdl(k_tree_attn_mma<T, STORE, HD>, dim3(static_cast<unsigned>(a.grid)), dim3(Z::THREADS), Z::SMEM, s, a, maps, kv_ptr<C>(cache, false),
+  STX_CUDA(launch_pdl(k_tree_attn_mma<T, STORE, HD, REP>, dim3(static_cast<unsigned>(a.grid)), dim3(Z::THREADS), Z::SMEM, s, a, maps, kv_ptr<C>(cache, false),
                       kv_ptr<C>(cache, true), vec));
   return launch_tree_join(a, TM_ROWS, Z::KT, cache->dtype, s);
 }
@@ -938,13 +958,15 @@ int tree_mma(TreeArgs a, const stx_kv* cache, cudaStream_t s) {
   a.grid = num_sms();
   auto ok = [](const void* p, int64_t x, int64_t y, int64_t z) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && x % 8 == 0 && y % 8 == 0 && z % 8 == 0; };
   const int vec = ok(a.q, a.q_seq, a.q_tok, a.q_head) && ok(a.out, a.o_seq, a.o_tok, a.o_head);
-  return by_store(cache->store, [&](auto st) -> int {
+  const bool few = a.tile_tok * a.group <= TM_ROWS / 4;
+  auto by_heads = [&](auto t, auto st) -> int {
+    typedef decltype(t) T;
     constexpr int S = decltype(st)::value;
-    if (cache->dtype == STX_F16)
-      return a.hd <= 64 ? launch_mma<__half, S, 64>(a, cache, o, vec, s) : a.hd <= 128 ? launch_mma<__half, S, 128>(a, cache, o, vec, s) : launch_mma<__half, S, 256>(a, cache, o, vec, s);
-    return a.hd <= 64 ? launch_mma<__nv_bfloat16, S, 64>(a, cache, o, vec, s)
-                      : a.hd <= 128 ? launch_mma<__nv_bfloat16, S, 128>(a, cache, o, vec, s) : launch_mma<__nv_bfloat16, S, 256>(a, cache, o, vec, s);
-  });
+    if (a.hd <= 64) return few ? launch_mma<T, S, 64, 4>(a, cache, o, vec, s) : launch_mma<T, S, 64, 1>(a, cache, o, vec, s);
+    if (a.hd <= 128) return few ? launch_mma<T, S, 128, 4>(a, cache, o, vec, s) : launch_mma<T, S, 128, 1>(a, cache, o, vec, s);
+    return few ? launch_mma<T, S, 256, 4>(a, cache, o, vec, s) : launch_mma<T, S, 256, 1>(a, cache, o, vec, s);
+  };
+  return by_store(cache->store, [&](auto st) -> int { return cache->dtype == STX_F16 ? by_heads(__half(), st) : by_heads(__nv_bfloat16(), st); });
 }
 
 }  // namespace stx
