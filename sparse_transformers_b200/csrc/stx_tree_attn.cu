@@ -183,80 +183,108 @@ __global__ void __launch_bounds__(TG_THREADS, 1) k_tree_attn_any(const TreeArgs 
 }
 
 constexpr int TJ_THREADS = 256;
-// Blocks (c, y): the unit that begins in CTA c's tiles and ends behind them; a thread has four values of a row.
-//   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the CTAs i = c, c + 1, .. that have a part of it, in that order,
-// eight parts' loads in flight at a time.  Lengths and counts are inputs of the launch before, which has waited for whoever wrote them:
-// the unit is found while that launch still runs.
+
+// Blocks (x, y): unit x, or, where there are more units than CTAs, the one that begins in CTA x's tiles and ends behind them.
+//   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the CTAs i = c, c + 1, .. that have a part of it
+// An item is four values of a row; P threads (2, 4 or 8, as there are parts) take every P-th part of it, four loads in flight each, and their
+// sums are added in thread order.  Lengths and counts are inputs of the launch before, which has waited for whoever wrote them, so the unit is found
+// while that launch still runs; a block without one leaves at once, all but one, so that this launch does not end before the one before it.
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const TreeArgs a, int kt) {
+__global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const TreeArgs a, int kt, int by_unit) {
   __shared__ int pre[TREE_MAX_SEQ + 1];
+  __shared__ float m_s[TJ_THREADS], l_s[TJ_THREADS];
+  __shared__ float4 o_s[TJ_THREADS];
   tree_prefix(a, kt, pre);
   __syncthreads();
   const TreeLine line = tree_line(a, pre);
-  const int cta = blockIdx.x;
-  bool mine = cta + 1 < line.ctas;
-  const int end = mine ? tree_begin(line, cta + 1) : 1, begin = mine ? tree_begin(line, cta) : 0;
-  const TreeSeg sg = tree_seg(a, line, pre, end - 1, end);
-  mine = mine && sg.first >= begin && sg.first + sg.nt > end;
-  const int rows = min(a.tile_tok, a.n_tok - sg.rt * a.tile_tok) * a.group;
-  const int item = blockIdx.y * TJ_THREADS + threadIdx.x, d4 = item / rows, row = item - d4 * rows;
-  const int tok = sg.rt * a.tile_tok + row / a.group;
-  mine = mine && 4 * d4 < a.hd;
-  const int parts = mine ? tree_owner(line, sg.first + sg.nt - 1) - cta + 1 : 0;
+  int at = 0;  // a position of the line in the unit
+  bool mine = true;
+  if (by_unit) {
+    const int b = blockIdx.x / line.per;
+    at = pre[b] * line.per + (blockIdx.x - b * line.per) * (pre[b + 1] - pre[b]);
+  } else {
+    mine = static_cast<int>(blockIdx.x) + 1 < line.ctas;
+    at = mine ? tree_begin(line, blockIdx.x + 1) - 1 : 0;
+  }
+  const TreeSeg sg = tree_seg(a, line, pre, at, at + 1);
+  const int cta = tree_owner(line, sg.first), begin = tree_begin(line, cta), parts = tree_owner(line, sg.first + sg.nt - 1) - cta + 1;
+  mine = mine && parts > 1 && (by_unit || cta == static_cast<int>(blockIdx.x));
+  if (!mine && (blockIdx.x | blockIdx.y)) return;
   pdl_wait();
   pdl_launch_dependents();
   if (!mine) return;
+  const int rows = min(a.tile_tok, a.n_tok - sg.rt * a.tile_tok) * a.group, items = rows * ((a.hd + 3) / 4);
   // CTA c ends with this unit: its first slot when the unit is all it has, else its second; those behind begin with it
   const int slot0 = 2 * cta + (sg.first == begin ? 0 : 1);
-  float M = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < parts; i0 += 8) {
-    float m[8], li[8];
-    float4 v[8];
+  const int P = parts <= 2 ? 2 : parts <= 4 ? 4 : 8, N = TJ_THREADS / P;
+  const int x = threadIdx.x & (N - 1), y = threadIdx.x / N;
+  for (int i0 = blockIdx.y * N; i0 < items; i0 += gridDim.y * N) {
+    const int item = i0 + x, d4 = item / rows, row = item - d4 * rows;
+    float M = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (item < items) {
+      for (int p0 = y; p0 < parts; p0 += 4 * P) {
+        float m[4], li[4];
+        float4 v[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int slot = i0 + k == 0 ? slot0 : 2 * (cta + i0 + k);
-      m[k] = -INFINITY;
-      li[k] = 0.f;
-      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i0 + k < parts) {
-        const float* ml = tree_part_ml(a, ROWS, slot);
-        m[k] = __ldcg(ml + row);
-        li[k] = __ldcg(ml + ROWS + row);
-        v[k] = __ldcg(reinterpret_cast<const float4*>(tree_part_o(a, ROWS, slot) + (static_cast<size_t>(d4) * ROWS + row) * 4));
+        for (int k = 0; k < 4; ++k) {
+          const int part = p0 + k * P, slot = part == 0 ? slot0 : 2 * (cta + part);
+          m[k] = -INFINITY;
+          li[k] = 0.f;
+          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (part < parts) {
+            const float* ml = tree_part_ml(a, ROWS, slot);
+            m[k] = __ldcg(ml + row);
+            li[k] = __ldcg(ml + ROWS + row);
+            v[k] = __ldcg(reinterpret_cast<const float4*>(tree_part_o(a, ROWS, slot) + (static_cast<size_t>(d4) * ROWS + row) * 4));
+          }
+        }
+        const float up = fmaxf(M, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+        const float f0 = M == up ? 1.f : exp2f(M - up);
+        M = up;
+        l *= f0, o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float f = m[k] == -INFINITY && li[k] == 0.f ? 0.f : exp2f(m[k] - M);  // a part that has seen nothing
+          l = fmaf(li[k], f, l), o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
+        }
       }
     }
-    float up = M;
+    m_s[threadIdx.x] = M;
+    l_s[threadIdx.x] = l;
+    o_s[threadIdx.x] = o;
+    __syncthreads();
+    if (y == 0 && item < items) {
+      float all = -INFINITY, sum = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < P; ++k) all = fmaxf(all, m_s[k * N + x]);
+      for (int k = 0; k < P; ++k) {
+        const float m = m_s[k * N + x], li = l_s[k * N + x], f = m == -INFINITY && li == 0.f ? 0.f : exp2f(m - all);
+        const float4 v = o_s[k * N + x];
+        sum = fmaf(li, f, sum);
+        r[0] = fmaf(v.x, f, r[0]), r[1] = fmaf(v.y, f, r[1]), r[2] = fmaf(v.z, f, r[2]), r[3] = fmaf(v.w, f, r[3]);
+      }
+      const int tok = sg.rt * a.tile_tok + row / a.group;
+      T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + tok * a.o_tok + (sg.head * a.group + row % a.group) * a.o_head + 4 * d4;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) up = fmaxf(up, m[k]);
-    const float f0 = M == up ? 1.f : exp2f(M - up);
-    M = up;
-    l *= f0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= f0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float f = m[k] == -INFINITY && li[k] == 0.f ? 0.f : exp2f(m[k] - M);  // a part that has seen nothing
-      l = fmaf(li[k], f, l);
-      o[0] = fmaf(v[k].x, f, o[0]);
-      o[1] = fmaf(v[k].y, f, o[1]);
-      o[2] = fmaf(v[k].z, f, o[2]);
-      o[3] = fmaf(v[k].w, f, o[3]);
+      for (int e = 0; e < 4; ++e)
+        if (4 * d4 + e < a.hd) dst[e] = DT<T>::from_f(all == -INFINITY && sum == 0.f ? 0.f : r[e] / sum);
     }
+    __syncthreads();
   }
-  T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + tok * a.o_tok + (sg.head * a.group + row % a.group) * a.o_head + 4 * d4;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (4 * d4 + e < a.hd) dst[e] = DT<T>::from_f(M == -INFINITY && l == 0.f ? 0.f : o[e] / l);
 }
 
 int launch_tree_join(const TreeArgs& a, int rows, int kt, int dtype, cudaStream_t s) {
+  const int64_t units = static_cast<int64_t>(a.n_seq) * a.nkv * a.row_tiles;
+  const int by_unit = units <= a.grid;
+  const int x = by_unit ? static_cast<int>(units) : a.grid;
+  // about four blocks an SM in all, and none without an item
   const int items = a.tile_tok * a.group * ((a.hd + 3) / 4);
-  const dim3 grid(static_cast<unsigned>(a.grid), static_cast<unsigned>((items + TJ_THREADS - 1) / TJ_THREADS));
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(std::max(1, std::min((items + 31) / 32, 4 * num_sms() / x))));
   return by_dtype(dtype, [&](auto tag) -> int {
     typedef decltype(tag) T;
-    if (rows == 16) STX_CUDA(launch_pdl(k_tree_join<T, 16>, grid, dim3(TJ_THREADS), 0, s, a, kt));
-    else if (rows == 64) STX_CUDA(launch_pdl(k_tree_join<T, 64>, grid, dim3(TJ_THREADS), 0, s, a, kt));
-    else STX_CUDA(launch_pdl(k_tree_join<T, 128>, grid, dim3(TJ_THREADS), 0, s, a, kt));
+    if (rows == 16) STX_CUDA(launch_pdl(k_tree_join<T, 16>, grid, dim3(TJ_THREADS), 0, s, a, kt, by_unit));
+    else if (rows == 64) STX_CUDA(launch_pdl(k_tree_join<T, 64>, grid, dim3(TJ_THREADS), 0, s, a, kt, by_unit));
+    else STX_CUDA(launch_pdl(k_tree_join<T, 128>, grid, dim3(TJ_THREADS), 0, s, a, kt, by_unit));
     return STX_OK;
   });
 }

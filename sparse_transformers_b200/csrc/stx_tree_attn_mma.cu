@@ -606,38 +606,44 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           ml[TM_ROWS + row] = sum;
         }
       }
-      // C columns at a time: every thread brings its half of them, scaled, to shared memory (over Q, which no product reads any more),
-      // [stream and lane group][column][row], and takes EL columns of a row from there.
+      // Every thread brings its columns, scaled, to shared memory, [stream and lane group][column][row], and takes EL columns of a row at a time from
+      // there: 32 columns in turn over Q, which no product reads any more, or, behind the CTA's last segment, all of them over the tiles.
       constexpr int C = 32, EL = RR * C / (32 * Z::SW);
-      float* xch = reinterpret_cast<float*>(q_t);
+      constexpr bool WIDE = NS * (DK + DV) * Z::TILE >= NS * TM_ROWS * HD * 4;
+      const bool last = WIDE && w.x + nt >= w.end;
+      const int cw = last ? HD : C;  // columns at a time
+      float* xch = reinterpret_cast<float*>(last ? k_t : q_t);
       const int orow = tid % RR, ocol = tid / RR * EL;
       const int otok = tok0 + orow / a.group;
       const unsigned long long bad = bad_s;
 #pragma unroll 1
-      for (int c0 = 0; c0 < HD; c0 += C) {
-        {
-          float* to = xch + ((st * REP + rep) * C + hf * (C / HF)) * RR + row;
+      for (int c0 = 0; c0 < HD; c0 += cw) {
+#pragma unroll 1
+        for (int c1 = 0; c1 < cw; c1 += C) {
+          float* to = xch + ((st * REP + rep) * cw + c1 + hf * (C / HF)) * RR + row;
           if (have && warp_used) {
             uint32_t r[C / HF];
-            tm_ld(o_addr + c0 + hf * (C / HF), r);
+            tm_ld(o_addr + c0 + c1 + hf * (C / HF), r);
 #pragma unroll
             for (int j = 0; j < C / HF; ++j) to[j * RR] = used ? __uint_as_float(r[j]) * f : 0.f;
           } else {
 #pragma unroll
             for (int j = 0; j < C / HF; ++j) to[j * RR] = 0.f;
           }
+          __syncwarp();
         }
-        __syncwarp();
         asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
-        const int col = c0 + ocol;
-        if (orow < rows && col < a.hd) {  // hd is a multiple of 8, and EL divides 8 or is a multiple of it
+#pragma unroll 1
+        for (int c1 = 0; c1 < cw; c1 += C) {
+          const int col = c0 + c1 + ocol;
+          if (orow >= rows || col >= a.hd) continue;  // hd is a multiple of 8, and EL divides 8 or is a multiple of it
           float o[EL];
           const float inv = inv_s[orow];
 #pragma unroll
           for (int j = 0; j < EL; ++j) {
             o[j] = 0.f;
 #pragma unroll
-            for (int k = 0; k < NS * REP; ++k) o[j] += xch[(k * C + ocol + j) * RR + orow];
+            for (int k = 0; k < NS * REP; ++k) o[j] += xch[(k * cw + c1 + ocol + j) * RR + orow];
             o[j] = inv == 0.f ? 0.f : o[j] * inv;
           }
           if (whole) {
@@ -653,7 +659,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           }
         }
         __syncwarp();
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
+        if (c0 + cw < HD) asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
       }
       tm_fence_before();
       __syncwarp();
