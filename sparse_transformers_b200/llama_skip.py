@@ -15,6 +15,11 @@ Weights are random (N(0, 0.02), seeded): checkpoints are not available offline.
 The decode step (all layers, lm_head, greedy argmax, KV-cache append, position advance) is
 captured once into a CUDA graph and replayed per token with no host synchronisation; each
 layer's cache maintenance runs on a side stream inside the same graph.
+
+``generate_speculative`` scores several drafted tokens per pass instead: their keys are rotated and
+written behind the sequence, the nodes attend to the cache and to their ancestors, the sparse MLP
+runs on the union of the nodes' active neurons, and the accepted path is kept.  ``kv_store`` holds
+the key/value cache in 8 bits for either way of decoding.
 """
 from __future__ import annotations
 
@@ -23,12 +28,16 @@ import math
 import time
 from dataclasses import dataclass
 from statistics import NormalDist
+from typing import Callable, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
 
 from . import _capi as C
+from .draft import draft_masks, tree_attention, verify_draft
+from .kv_cache import KVCache
 from .layer import SparseLayer
+from .rope import RotaryPositions
 
 
 @dataclass
@@ -55,6 +64,9 @@ class LlamaSkipConfig:
     # measured 7 % slower there than stx_add_rmsnorm followed by the torch matmul, so it is off by default
     qkv_proj: str = "torch"        # "torch" | "gemv" (stx_add_rmsnorm, then stx_norm_gemv without norm) | "fused"
     own_wo: bool = True
+    kv_store: str = "same"         # key/value cache: "same" (dtype) | "int8" | "e4m3" (codes and a scale per row)
+    rope_scaling: Optional[dict] = None  # as RotaryPositions takes it; None: plain rotary positions
+    draft_nodes: int = 0           # generate_speculative: most nodes of a draft, its root included (64 at most)
 
     @property
     def tau(self) -> float:
@@ -122,6 +134,17 @@ def rope_tables(cfg: LlamaSkipConfig, device) -> tuple[torch.Tensor, torch.Tenso
     return emb.cos(), emb.sin()  # [max_len, head_dim] fp32
 
 
+def prompt_lookup(tokens: Sequence[int], n: int, ngram: int = 3) -> list[int]:
+    """Up to n tokens that followed the latest earlier occurrence of the last ``ngram`` tokens, or of fewer of them."""
+    tokens = list(tokens)
+    for m in range(min(ngram, len(tokens) - 1), 0, -1):
+        tail = tokens[-m:]
+        for at in range(len(tokens) - m - 1, -1, -1):
+            if tokens[at:at + m] == tail:
+                return tokens[at + m:at + m + n]
+    return []
+
+
 def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
     """x [heads, T, hd]; cos/sin [T, hd] (rotate-half convention)."""
     h = x.shape[-1] // 2
@@ -138,6 +161,8 @@ class LlamaSkipModel:
         def rn(*shape):
             return (torch.randn(*shape, generator=g, device=self.device, dtype=torch.float32) * cfg.wstd).to(dt)
 
+        if not 0 <= cfg.draft_nodes <= C.DRAFT_MAX:
+            raise ValueError(f"draft_nodes must be 0..{C.DRAFT_MAX}, not {cfg.draft_nodes}")
         H, I, hd = cfg.hidden, cfg.intermediate, cfg.head_dim
         self.embed = rn(cfg.vocab, H)          # tied with lm_head, as Llama-3.2 does
         self.final_norm = torch.ones(H, dtype=dt, device=self.device)
@@ -148,12 +173,13 @@ class LlamaSkipModel:
                 ln1=torch.ones(H, dtype=dt, device=self.device), ln2=torch.ones(H, dtype=dt, device=self.device),
                 gate=rn(I, H), up=rn(I, H), down=rn(H, I), A=rn(cfg.predictor_rank, H), Bm=rn(I, cfg.predictor_rank))
             L["sparse"] = SparseLayer(L["gate"], L["up"], L["down"], L["A"], L["Bm"], act=cfg.act, method="threshold",
-                                      param=cfg.tau, max_batch=1, alias_gate_up=True, init_all_active=True,
+                                      param=cfg.tau, max_batch=max(1, cfg.draft_nodes), alias_gate_up=True, init_all_active=True,
                                       lazy_cache=cfg.lazy_cache)
             self.layers.append(L)
-        self.cos, self.sin = rope_tables(cfg, self.device)
-        self.k_cache = torch.zeros(cfg.layers, cfg.kv_heads, cfg.max_len, hd, dtype=dt, device=self.device)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.rope = RotaryPositions(hd, theta=cfg.rope_theta, scaling=cfg.rope_scaling, device=self.device)
+        self.cos, self.sin = rope_tables(cfg, self.device) if cfg.rope_scaling is None else self.rope.tables(cfg.max_len)
+        self.kv = KVCache(1, cfg.kv_heads, cfg.max_len, hd, dtype=dt, store=cfg.kv_store, layers=cfg.layers, device=self.device)
+        self.k_cache, self.v_cache = self.kv.k[:, 0], self.kv.v[:, 0]  # [layers, kv_heads, max_len, head_dim]
         # decode state, all on the device so that the captured step needs no host input
         self.pos = torch.zeros(1, dtype=torch.long, device=self.device)
         self.gen_base = torch.zeros(1, dtype=torch.long, device=self.device)  # prompt length of the current generation
@@ -166,12 +192,15 @@ class LlamaSkipModel:
         self._attn_ws = attn_workspace(cfg.heads, cfg.head_dim, self.device)
         self._finish_ws = torch.zeros(16, dtype=torch.uint8, device=self.device)
         self._graph = None
+        self._draft_graphs = {}  # (nodes, tree, sampled) -> captured pass over a draft
         self.trace = None  # when a list: per decode step and layer (x_pred, x_mlp, mlp_out, mask) copies, eager mode only
 
     # ------------------------------------------------------------------ pieces
     def _attention(self, li: int, x: torch.Tensor, pos0, T: int, decode: bool) -> torch.Tensor:
         cfg, L = self.cfg, self.layers[li]
         hd, nh, nkv = cfg.head_dim, cfg.heads, cfg.kv_heads
+        if decode and cfg.kv_store != "same":
+            return self._attention_cached(li, x, self.pos, None, None)
         qkv = x @ L["wqkv"].t()                                                  # [T, (nh+2nkv)*hd]
         q, k, v = qkv.split([nh * hd, nkv * hd, nkv * hd], dim=-1)
         q = q.view(T, nh, hd).transpose(0, 1)
@@ -189,11 +218,25 @@ class LlamaSkipModel:
         else:
             cos, sin = self.cos[pos0:pos0 + T], self.sin[pos0:pos0 + T]
             q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
-            self.k_cache[li, :, pos0:pos0 + T] = k
-            self.v_cache[li, :, pos0:pos0 + T] = v
+            if cfg.kv_store == "same":
+                self.k_cache[li, :, pos0:pos0 + T] = k
+                self.v_cache[li, :, pos0:pos0 + T] = v
+            else:                                                                # the prompt attends to its own exact rows
+                start = torch.full((1,), pos0, dtype=torch.long, device=self.device)
+                self.kv.layer(li).append(k.transpose(0, 1).unsqueeze(0), v.transpose(0, 1).unsqueeze(0), start)
             o = F.scaled_dot_product_attention(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), is_causal=True, enable_gqa=True)
         o = o.squeeze(0).transpose(0, 1).reshape(T, nh * hd)
         return o @ L["wo"].t()
+
+    def _attention_cached(self, li: int, x: torch.Tensor, start: torch.Tensor, positions: Optional[torch.Tensor],
+                          masks: Optional[torch.Tensor]) -> torch.Tensor:
+        """Attention of the nodes x [n,H] that stand in slots start[0] + i: rotate and write, then attend to the cache."""
+        cfg, L, n = self.cfg, self.layers[li], x.shape[0]
+        qkv = (x @ L["wqkv"].t()).view(1, n, cfg.heads + 2 * cfg.kv_heads, cfg.head_dim)
+        q, k, v = qkv.split([cfg.heads, cfg.kv_heads, cfg.kv_heads], dim=2)
+        kv = self.kv.layer(li)
+        q = kv.append(k, v, start, rope=self.rope, positions=positions, q=q, q_out=q)
+        return tree_attention(q, kv, start, tree=masks).view(n, -1) @ L["wo"].t()
 
     def _dense_mlp(self, li: int, x: torch.Tensor) -> torch.Tensor:
         L = self.layers[li]
@@ -269,7 +312,7 @@ class LlamaSkipModel:
 
     def _decode_body(self) -> None:
         cfg = self.cfg
-        if cfg.native_glue and cfg.head_dim in (64, 128, 256) and cfg.max_len <= 8192:
+        if cfg.native_glue and cfg.kv_store == "same" and cfg.head_dim in (64, 128, 256) and cfg.max_len <= 8192:
             return self._decode_body_native()
         main = torch.cuda.current_stream()
         h = self.embed.index_select(0, self.token)                              # [1,H]
@@ -336,7 +379,121 @@ class LlamaSkipModel:
         return {"tokens": self.generated[:n_new].clone(), "ttft_s": t1 - t0, "decode_s": t2 - t1,
                 "output_tokens_per_s": (n_new - 1) / (t2 - t1), "total_tokens_per_s": n_new / (t2 - t0)}
 
+    # ------------------------------------------------------------------ several drafted tokens per pass
+    def _draft_body(self, tokens: torch.Tensor, parents: Optional[torch.Tensor], uniform: Optional[torch.Tensor],
+                    temperature: float) -> torch.Tensor:
+        """One pass over a draft tokens [1,n] whose root is the settled token in slot pos: keeps the accepted path in the
+        cache, advances pos and token, returns path, count and the next token as one int64 vector [n + 2]."""
+        cfg = self.cfg
+        h = self.embed.index_select(0, tokens[0])                               # [n,H]
+        start = self.pos.clone()
+        masks, positions = None, None                                           # of a chain: everything before, slot by slot
+        if parents is not None:
+            masks, depth = draft_masks(parents)
+            positions = depth + start[:, None]
+        for li, L in enumerate(self.layers):
+            x_pred = rms_norm(h, L["ln1"], cfg.rms_eps)
+            h = h + self._attention_cached(li, x_pred, start, positions, masks)
+            h = h + L["sparse"].step(x_pred, rms_norm(h, L["ln2"], cfg.rms_eps))
+        logits = (rms_norm(h, self.final_norm, cfg.rms_eps) @ self.embed.t()).float()
+        if uniform is None:
+            path, count, nxt = verify_draft(tokens, logits.argmax(-1).unsqueeze(0), parents=parents)
+        else:
+            path, count, nxt = verify_draft(tokens, torch.softmax(logits / temperature, -1).unsqueeze(0), uniform=uniform, parents=parents)
+        if parents is not None:
+            self.kv.keep(start, path, count)                                    # a chain's path lies in place already
+        self.pos.add_(count)
+        self.token.copy_(nxt)
+        return torch.cat([path[0], count, nxt])
+
+    def _draft_pass(self, tokens: list[int], parents: Optional[list[int]], uniform: Optional[torch.Tensor], temperature: float,
+                    use_graph: bool) -> list[int]:
+        n = len(tokens)
+        host = torch.tensor([tokens, parents or [0] * n], dtype=torch.long)
+        if not use_graph:
+            dev = host.to(self.device)
+            return self._draft_body(dev[:1], dev[1:] if parents else None, uniform, temperature).tolist()
+        key = (n, parents is not None, temperature if uniform is not None else None)
+        if key not in self._draft_graphs:
+            dev = host.to(self.device)
+            u = None if uniform is None else uniform.clone()
+            args = (dev[:1], dev[1:] if parents else None, u, temperature)
+            state = (self.pos.clone(), self.token.clone(), self.generated.clone())
+            s = torch.cuda.Stream(device=self.device)
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                self._draft_body(*args)                                          # allocator, function attributes
+            torch.cuda.current_stream().wait_stream(s)
+            torch.cuda.synchronize()
+            self._restore(state)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = self._draft_body(*args)
+            self._restore(state)                                                 # the slots behind pos are written anew below
+            self._draft_graphs[key] = (g, dev, u, out)
+        g, dev, u, out = self._draft_graphs[key]
+        dev.copy_(host)
+        if u is not None:
+            u.copy_(uniform)
+        g.replay()
+        return out.tolist()
+
+    @torch.no_grad()
+    def generate_speculative(self, prompt_ids: torch.Tensor, n_new: int, draft: Optional[Callable] = None, *, temperature: float = 0.0,
+                             seed: int = 0, use_graph: bool = True) -> dict:
+        """Decoding from drafted tokens: the result follows the model's greedy choices (temperature 0) or its distribution at
+        ``temperature``, whatever is drafted.  The active neurons of a pass are the union over its nodes, so at densities below 1
+        a token's MLP runs on a superset of the neurons that ``generate`` gives it.
+
+        draft(tokens, n): the tokens so far (prompt and new ones, a list) and the most nodes that may be drafted -> the tokens
+        that may follow, a chain; or (tokens, parents), a tree: parents[i] < i is the drafted node before node i, -1 the last
+        token so far.  Default: prompt_lookup.  Returns what ``generate`` returns, and ``passes`` and ``accepted`` (drafted tokens
+        that were kept)."""
+        cfg = self.cfg
+        if cfg.draft_nodes < 1:
+            raise ValueError("generate_speculative needs draft_nodes of at least 1 in the model's configuration")
+        if temperature < 0:
+            raise ValueError(f"temperature must not be negative, not {temperature}")
+        draft = draft or prompt_lookup
+        T = int(prompt_ids.numel())
+        if T < 1 or n_new < 1 or T + n_new > cfg.max_len:
+            raise ValueError(f"a prompt of {T} and {n_new} new tokens in a cache of {cfg.max_len}")
+        gen = torch.Generator(device=self.device).manual_seed(seed)
+        draw = lambda n: torch.rand(1, n, generator=gen, device=self.device) if temperature > 0 else None
+        tokens = prompt_ids.tolist()
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        first = self.prefill(prompt_ids)
+        if temperature > 0:                                                      # the root of a draft of one node, drawn
+            first = verify_draft(prompt_ids[-1:].view(1, 1), torch.softmax(self.logits / temperature, -1).view(1, 1, -1), uniform=draw(1))[2]
+            self.token.copy_(first)
+        tokens.append(int(first))
+        t1 = time.perf_counter()
+        passes = accepted = 0
+        while len(tokens) < T + n_new:
+            room = min(cfg.draft_nodes - 1, T + n_new - len(tokens) - 1)         # a pass emits one token more than it keeps
+            ids = draft(list(tokens), room) if room else []
+            ids, parents = ids if isinstance(ids, tuple) else (ids, None)
+            ids = [int(t) for t in ids]
+            if len(ids) > room or any(not 0 <= t < cfg.vocab for t in ids):
+                raise ValueError(f"draft gave {len(ids)} tokens where {room} may be drafted, or one outside the vocabulary")
+            if parents is not None:
+                parents = [int(p) for p in parents]
+                if len(parents) != len(ids) or any(not -1 <= p < i for i, p in enumerate(parents)):
+                    raise ValueError("draft's parents must name an earlier drafted node each, or -1")
+                parents = [-1] + [p + 1 for p in parents]
+            nodes = [tokens[-1]] + ids
+            got = self._draft_pass(nodes, parents, draw(len(nodes)), temperature, use_graph)
+            count, nxt = got[-2:]
+            tokens += [nodes[i] for i in got[1:count]] + [nxt]
+            passes, accepted = passes + 1, accepted + count - 1
+        t2 = time.perf_counter()
+        new = torch.tensor(tokens[T:], dtype=torch.long, device=self.device)
+        return {"tokens": new, "ttft_s": t1 - t0, "decode_s": t2 - t1, "output_tokens_per_s": (n_new - 1) / (t2 - t1),
+                "total_tokens_per_s": n_new / (t2 - t0), "passes": passes, "accepted": accepted}
+
     def close(self) -> None:
         self._graph = None
+        self._draft_graphs = {}
         for L in self.layers:
             L["sparse"].close()

@@ -129,3 +129,14 @@ def test_cpu_tensors_and_bad_caches_are_refused():
               lambda: KVCache.from_tensors(torch.zeros(1, 2, 3), torch.zeros(1, 2, 3)), lambda: KVCache.from_tensors(*[torch.zeros(1, 1, 1, 8, dtype=torch.int8)] * 2)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_prompt_lookup():
+    from sparse_transformers_b200.llama_skip import prompt_lookup
+
+    assert prompt_lookup([1, 2, 3, 9, 1, 2, 3], 2) == [9, 1]
+    assert prompt_lookup([1, 2, 3, 9, 1, 2, 3], 0) == []
+    assert prompt_lookup([4, 5, 6], 3) == []
+    assert prompt_lookup([7], 3) == [] and prompt_lookup([], 3) == []
+    assert prompt_lookup([8, 1, 5, 8, 2, 6, 8], 1) == [2]             # the latest occurrence
+    assert prompt_lookup([8, 8], 4) == [8]
