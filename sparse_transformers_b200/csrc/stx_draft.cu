@@ -80,7 +80,7 @@ __device__ __forceinline__ void vf_walk(const float* p, const float* q, int64_t 
   }
 }
 
-__global__ void __launch_bounds__(VF_THREADS, 1) k_verify_walk(const VerifyArgs a, int seg, int vec) {
+__global__ void __launch_bounds__(VF_THREADS, 2) k_verify_walk(const VerifyArgs a, int seg, int vec) {
   __shared__ double tot_s[2][VF_SEGS];  // sums of the cluster's stretches, two draws in turn
   __shared__ int tok_s[2];
   __shared__ int64_t x_s[STX_DRAFT_MAX], par_s[STX_DRAFT_MAX];
