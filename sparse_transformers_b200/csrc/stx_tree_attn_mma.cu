@@ -450,7 +450,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       {
         const T* src = static_cast<const T*>(a.q) + sg.b * a.q_seq + tok * a.q_tok + head * a.q_head;
         const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale goes with Q
-        constexpr int MINE = HD / 8 / (HF * NS), BATCH = MINE < 4 ? MINE : 4;  // 16-byte pieces of a row, requested together
+        constexpr int MINE = HD / 8 / (HF * NS), BATCH = MINE < 8 ? MINE : 8;  // 16-byte pieces of a row, requested together
 #pragma unroll 1
         for (int c0 = 0; c0 < MINE; c0 += BATCH) {
           uint4 v[BATCH];
@@ -787,10 +787,10 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         ok = ok && tm_wait(&r_full[rs], ruse & 1, dead);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        constexpr int PER = HD / 16, EACH = KT * PER / CT, BATCH = EACH < 4 ? EACH : 4;  // 16-byte pieces of a row of codes, of a thread
+        constexpr int PER = HD / 16, EACH = KT * PER / CT, BATCH = EACH < 2 ? EACH : 2;  // 16-byte pieces of a row of codes, of a thread
         const unsigned char* src = raw + rs * Z::RAW_TILE;
         unsigned char* dst = tiles_t + s * Z::TILE;
-#pragma unroll
+#pragma unroll 1
         for (int i0 = 0; i0 < EACH; i0 += BATCH) {
           uint4 w4[BATCH];
 #pragma unroll
@@ -798,7 +798,9 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
             const int at = ct + CT * (i0 + i), r = at / PER, piece = at % PER;
-            const uint32_t q4[4] = {w4[i].x, w4[i].y, w4[i].z, w4[i].w};
+            // Eight lanes store at a time, of a row's two parts that lie in the same banks: those of the second part their upper half first.
+            const int up = (piece >> 2) & 1;
+            const uint32_t q4[4] = {up ? w4[i].z : w4[i].x, up ? w4[i].w : w4[i].y, up ? w4[i].x : w4[i].z, up ? w4[i].y : w4[i].w};
             uint32_t e[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) e[k] = tm_operand<T, STORE>(q4[k / 2], k & 1);
@@ -810,9 +812,9 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
               }
             }
             unsigned char* to = dst + (piece >> 2) * Z::BOX + r * 128;
-            const int ch = (piece & 3) * 2;
+            const int ch = (piece & 3) * 2 + up;
             *reinterpret_cast<uint4*>(to + ((ch ^ (r & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
-            *reinterpret_cast<uint4*>(to + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
+            *reinterpret_cast<uint4*>(to + ((ch ^ 1 ^ (r & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
           }
         }
         tm_fence_async();
