@@ -62,7 +62,7 @@ template <int STORE, int HD, int REP> struct TmShape {
   static constexpr uint32_t QX = Q < 32768 ? 32768 : Q;  // Q, later the exchange of a segment's end
   static constexpr uint32_t SMEM_TILES = QX + NS * (DK + DV) * TILE + 2 * RAW * RAW_TILE;
   static constexpr uint32_t SMEM_SCALES = CODED ? NS * SCALES * 3 * KT * 4 : 0;
-  static constexpr uint32_t SMEM_ML = 3 * HF * NS * TM_ROWS * 4;  // m (of tile and segment) and l of each thread of the soft-max
+  static constexpr uint32_t SMEM_ML = 2 * HF * NS * TM_ROWS * 4;  // m of a tile, two in turn; at a segment's end its m and l
   static constexpr uint32_t BARS = 2 * NS * (DK + DV) + 2 * NB + 4 * NS + 4 * RAW + (CODED ? NS * SCALES : 0);
   static constexpr uint32_t SMEM = 1024 + SMEM_TILES + SMEM_SCALES + SMEM_ML + BARS * 8 + 64;
   static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1 + TM_ROWS) + 64 <= 227 * 1024, "shared memory of a CTA");
@@ -362,7 +362,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   unsigned char* v_t = k_t + NS * DK * Z::TILE;
   unsigned char* raw_t = v_t + NS * DV * Z::TILE;
   float* sc_s = reinterpret_cast<float*>(raw_t + 2 * Z::RAW * Z::RAW_TILE);  // [SCALES][3][KT]
-  float* ml_s = sc_s + Z::SMEM_SCALES / 4;  // m of a tile, two in turn [2][HF NS][TM_ROWS] (the first also: m of a segment), l [HF NS][TM_ROWS]
+  float* ml_s = sc_s + Z::SMEM_SCALES / 4;  // [2][HF NS][TM_ROWS]
   uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + Z::SMEM_ML / 4);
   uint64_t *k_full = bars, *k_empty = k_full + NS * DK, *v_full = k_empty + NS * DK, *v_empty = v_full + NS * DV, *s_full = v_empty + NS * DV;
   uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + NS, *raw_full = drain + NS;
@@ -577,89 +577,121 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
       }
       asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");  // bad_s of all warps; every product of the segment is done, every maximum read
       ml_s[who * TM_ROWS + tl] = m;
-      ml_s[(2 * HF * NS + who) * TM_ROWS + tl] = l;
+      ml_s[(HF * NS + who) * TM_ROWS + tl] = l;
+      tm_fence_before();
       asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
-      // The row's results, NS streams x REP lane groups: M, and each one's share of the sum, 2^(m - M), in the same order everywhere.
-      float big = m;
+      tm_fence_after();
+      // The row's results, NS streams x REP lane groups: M, each one's factor 2^(m - M), and the sum, in the same order everywhere.
+      float big = -INFINITY, sum = 0.f, f[NS];
 #pragma unroll
       for (int k = 0; k < NS * REP; ++k) big = fmaxf(big, ml_s[HF * (k / REP) * TM_ROWS + (k % REP) * RR + row]);
-      const float f = m == big ? 1.f : exp2f(m - big);
+#pragma unroll
+      for (int k = 0; k < NS * REP; ++k) {
+        const int at = HF * (k / REP) * TM_ROWS + (k % REP) * RR + row;
+        const float mk = ml_s[at];
+        float lk = ml_s[HF * NS * TM_ROWS + at];
+        if (HF == 2) lk += ml_s[(HF * NS + 1) * TM_ROWS + at];
+        sum += lk * (mk == big ? 1.f : exp2f(mk - big));
+      }
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        const float mk = ml_s[HF * k * TM_ROWS + tl];
+        f[k] = mk == big ? 1.f : exp2f(mk - big);
+      }
       const bool gone = !ok || *dead;
       const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
       const int slot = 2 * cta + (w.x == begin ? 0 : 1);
       float* po = tree_part_o(a, TM_ROWS, slot);
+      // 1 / l; 0 where nothing was seen (what weights of zero met does not count), NaN where a wait has expired
+      const float inv_row = gone ? __int_as_float(0x7fc00000) : big == -INFINITY && sum == 0.f ? 0.f : whole ? 1.f / sum : 1.f;
       if (who == 0 && rep == 0) {
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < NS * REP; ++k) {
-          const int at = HF * (k / REP) * TM_ROWS + (k % REP) * RR + row;
-          const float mk = ml_s[at];
-          float lk = ml_s[2 * HF * NS * TM_ROWS + at];
-          if (HF == 2) lk += ml_s[(2 * HF * NS + 1) * TM_ROWS + at];
-          sum += lk * (mk == big ? 1.f : exp2f(mk - big));
-        }
-        // 1 / l; 0 where nothing was seen (what weights of zero met does not count), NaN where a wait has expired
-        inv_s[row] = gone ? __int_as_float(0x7fc00000) : big == -INFINITY && sum == 0.f ? 0.f : whole ? 1.f / sum : 1.f;
+        inv_s[row] = inv_row;
         if (!whole) {
           float* ml = tree_part_ml(a, TM_ROWS, slot);
           ml[row] = big;
           ml[TM_ROWS + row] = sum;
         }
       }
-      // Every thread brings its columns, scaled, to shared memory, [stream and lane group][column][row], and takes EL columns of a row at a time from
-      // there: 32 columns in turn over Q, which no product reads any more, or, behind the CTA's last segment, all of them over the tiles.
-      constexpr int C = 32, EL = RR * C / (32 * Z::SW);
-      constexpr bool WIDE = NS * (DK + DV) * Z::TILE >= NS * TM_ROWS * HD * 4;
-      const bool last = WIDE && w.x + nt >= w.end;
-      const int cw = last ? HD : C;  // columns at a time
-      float* xch = reinterpret_cast<float*>(last ? k_t : q_t);
-      const int orow = tid % RR, ocol = tid / RR * EL;
-      const int otok = tok0 + orow / a.group;
       const unsigned long long bad = bad_s;
-#pragma unroll 1
-      for (int c0 = 0; c0 < HD; c0 += cw) {
-#pragma unroll 1
-        for (int c1 = 0; c1 < cw; c1 += C) {
-          float* to = xch + ((st * REP + rep) * cw + c1 + hf * (C / HF)) * RR + row;
-          if (have && warp_used) {
-            uint32_t r[C / HF];
-            tm_ld(o_addr + c0 + c1 + hf * (C / HF), r);
+      const uint32_t o_row = lane_base + Z::O_COL;
+      // N columns of the thread's row, added over the streams
+      auto gather = [&](int col, auto& o) {
+        constexpr int N = sizeof(o) / sizeof(float);
+        if (warp_used) {
+          uint32_t r[N];
+          tm_ld(o_row + col, r);
 #pragma unroll
-            for (int j = 0; j < C / HF; ++j) to[j * RR] = used ? __uint_as_float(r[j]) * f : 0.f;
-          } else {
+          for (int k = 0; k < N; ++k) o[k] = used ? __uint_as_float(r[k]) * f[0] : 0.f;
+          if (NS == 2 && nt > 1) {
+            tm_ld(o_row + HD + col, r);
 #pragma unroll
-            for (int j = 0; j < C / HF; ++j) to[j * RR] = 0.f;
+            for (int k = 0; k < N; ++k) o[k] += used ? __uint_as_float(r[k]) * f[NS - 1] : 0.f;
           }
-          __syncwarp();
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
-#pragma unroll 1
-        for (int c1 = 0; c1 < cw; c1 += C) {
-          const int col = c0 + c1 + ocol;
-          if (orow >= rows || col >= a.hd) continue;  // hd is a multiple of 8, and EL divides 8 or is a multiple of it
-          float o[EL];
-          const float inv = inv_s[orow];
+        } else {
 #pragma unroll
-          for (int j = 0; j < EL; ++j) {
-            o[j] = 0.f;
-#pragma unroll
-            for (int k = 0; k < NS * REP; ++k) o[j] += xch[(k * cw + c1 + ocol + j) * RR + orow];
-            o[j] = inv == 0.f ? 0.f : o[j] * inv;
-          }
-          if (whole) {
-            T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + otok * a.o_tok + (sg.head * a.group + orow % a.group) * a.o_head + col;
-            tm_store<T, EL>(dst, vec, o, a.hd - col);
-            if (bad) tm_add_bad<T, STORE>(dst, 1, bad & tree_bits(a, sq, sg.b, otok), vc, sg.b, sg.head, sq.len, col, min(EL, a.hd - col));
-          } else {
-#pragma unroll
-            for (int j = 0; j < EL; j += 2)
-              if (col + j < a.hd)
-                *reinterpret_cast<float2*>(po + (static_cast<size_t>((col + j) / 4) * TM_ROWS + orow) * 4 + (col + j) % 4) = make_float2(o[j], o[j + 1]);
-            if (bad) tm_add_bad<T, STORE>(po + static_cast<size_t>(orow) * 4, TM_ROWS, bad & tree_bits(a, sq, sg.b, otok), vc, sg.b, sg.head, sq.len, col, min(EL, a.hd - col));
-          }
+          for (int k = 0; k < N; ++k) o[k] = 0.f;
         }
         __syncwarp();
-        if (c0 + cw < HD) asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
+      };
+      // and N finished ones to their place
+      auto put = [&](int orow, int col, auto& o, float inv) {
+        constexpr int N = sizeof(o) / sizeof(float);
+        if (orow >= rows || col >= a.hd) return;  // hd is a multiple of 8
+        const int otok = tok0 + orow / a.group;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[k] = inv == 0.f ? 0.f : o[k] * inv;
+        if (whole) {
+          T* dst = static_cast<T*>(a.out) + sg.b * a.o_seq + otok * a.o_tok + (sg.head * a.group + orow % a.group) * a.o_head + col;
+          tm_store<T, N>(dst, vec, o, a.hd - col);
+          if (bad) tm_add_bad<T, STORE>(dst, 1, bad & tree_bits(a, sq, sg.b, otok), vc, sg.b, sg.head, sq.len, col, min(N, a.hd - col));
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; k += 4)
+            if (col + k < a.hd) *reinterpret_cast<float4*>(po + (static_cast<size_t>((col + k) / 4) * TM_ROWS + orow) * 4) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          if (bad) tm_add_bad<T, STORE>(po + static_cast<size_t>(orow) * 4, TM_ROWS, bad & tree_bits(a, sq, sg.b, otok), vc, sg.b, sg.head, sq.len, col, min(N, a.hd - col));
+        }
+      };
+      if constexpr (REP == 1) {  // a row's threads have a part of its columns each
+        constexpr int CS = HD / (HF * NS);
+#pragma unroll 1
+        for (int c0 = who * CS; c0 < (who + 1) * CS; c0 += 16) {
+          float o[16];
+          gather(c0, o);
+          put(row, c0, o, inv_row);
+          __syncwarp();
+        }
+      } else {
+        // The lane groups' sums meet in shared memory, [lane group][column][row]: over Q, which no product reads any more, as many columns as
+        // fit, or, behind the CTA's last segment, all of them over the tiles.  A warp takes eight columns of all rows at a time from there.
+        constexpr int FIT = Z::QX / (TM_ROWS * 4) < HD ? Z::QX / (TM_ROWS * 4) : HD;
+        constexpr bool WIDE = NS * (DK + DV) * Z::TILE >= TM_ROWS * HD * 4;
+        const bool last = WIDE && w.x + nt >= w.end;
+        const int cw = last ? HD : FIT;  // columns at a time
+        float* xch = reinterpret_cast<float*>(last ? k_t : q_t);
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD; c0 += cw) {
+#pragma unroll 1
+          for (int c1 = who * (cw / NS); c1 < (who + 1) * (cw / NS); c1 += 32) {
+            float o[32];
+            gather(c0 + c1, o);
+            float* to = xch + (rep * cw + c1) * RR + row;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) to[k * RR] = o[k];
+          }
+          asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
+#pragma unroll 1
+          for (int c1 = 8 * warp; c1 < cw; c1 += 8 * Z::SW) {
+            float o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float* from = xch + (c1 + k) * RR + lane;
+              o[k] = (from[0] + from[cw * RR]) + (from[2 * cw * RR] + from[3 * cw * RR]);
+            }
+            put(lane, c0 + c1, o, inv_s[lane]);
+            __syncwarp();
+          }
+          if (c0 + cw < HD) asm volatile("bar.sync 1, %0;" ::"n"(32 * Z::SW) : "memory");
+        }
       }
       tm_fence_before();
       __syncwarp();
