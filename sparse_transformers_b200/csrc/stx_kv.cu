@@ -37,6 +37,11 @@ int check_heads(const stx_heads* h, const char* who, const char* name) {
 
 constexpr int ROPE_THREADS = 256;
 
+// a / b of numbers that are not negative: a division of 64 bits costs about 100 instructions, as much as a row's other work.
+__device__ __forceinline__ int64_t quick_div(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
 // One launch of the rotation: q rows (heads 0 .. nh-1 of a token), then k and v rows where there is a cache.
 template <typename T, int STORE> struct RopeArgs {
   typedef typename Held<T, STORE>::C C;
@@ -124,12 +129,12 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_vec(const RopeArgs<T, STO
   const int64_t id = static_cast<int64_t>(blockIdx.x) * ROPE_THREADS + threadIdx.x;
   const int j = threadIdx.x % LPR;
   const int64_t row = id / LPR;
-  const int64_t tok = row / a.groups;
+  const int64_t tok = quick_div(row, a.groups);
   pdl_wait();
   pdl_launch_dependents();
   if (tok >= a.tokens) return;  // the lanes of a row leave together
   const int h0 = static_cast<int>(row - tok * a.groups);
-  const int64_t b = tok / a.n_tok, t = tok - b * a.n_tok;
+  const int64_t b = quick_div(tok, a.n_tok), t = tok - b * a.n_tok;
   const bool used = !a.counts || t < a.counts[b];
   const bool act = 16 * j < a.hd;
   const bool turned = 16 * j < a.rot;
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(256) k_kv_read_vec(const KvPtr<typename Held<T
   pdl_launch_dependents();
   if (id >= items) return;
   const int lpr = hd / 16;
-  const int64_t row = id / lpr, bh = row / n, b = bh / nkv;
+  const int64_t row = quick_div(id, lpr), bh = quick_div(row, n), b = quick_div(bh, nkv);
   const int j = static_cast<int>(id - row * lpr), h = static_cast<int>(bh - b * nkv);
   const int64_t slot = (start ? start[b] : 0) + row - bh * n;
   const bool there = slot >= 0 && slot < max_len;
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(256) k_kv_read_any(const KvPtr<typename Held<T
   pdl_wait();
   pdl_launch_dependents();
   if (id >= items) return;
-  const int64_t row = id / hd, bh = row / n, b = bh / nkv;
+  const int64_t row = quick_div(id, hd), bh = quick_div(row, n), b = quick_div(bh, nkv);
   const int d = static_cast<int>(id - row * hd), h = static_cast<int>(bh - b * nkv);
   const int64_t slot = (start ? start[b] : 0) + row - bh * n;
   const KvPtr<typename Held<T, STORE>::C>& c = blockIdx.y ? vc : kc;
