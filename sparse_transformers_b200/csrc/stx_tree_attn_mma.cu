@@ -1,26 +1,37 @@
 // stx_tree_attention on the 5th-generation tensor cores: fp16 and bf16 models, caches of 16 or 8 bits.
 //
-// A CTA per SM walks its segments (stx_tree_attn.cuh): up to 128 rows (tokens x query heads of a cache head) against tiles of KT
+// A CTA per SM walks its segments (stx_tree_attn.cuh): up to 128 rows (tokens x query heads of a cache head) against tiles of KT = 64
 // slots.  Per tile
 //   S = Q K^T      tcgen05.mma, 128 x KT, both operands in shared memory (128-byte swizzle), S in tensor memory
-//   P = 2^(S c - m)  softmax warps: a thread has a row; P goes back to tensor memory in the model's type
+//   P = 2^(S c - m)  soft-max warps; P goes back to tensor memory in the model's type: one rounding of a weight, half a step
 //   O += P V       tcgen05.mma, P from tensor memory, V as it lies in the cache ([slots][head_dim] is an MN-major operand)
 // With heads of up to 128 two streams of tiles (even and odd ones of the segment) with S, O, m and l of their own share the CTA:
 // while one's soft-max runs, the other one's products do, and neither waits for the other before the segment's end, where
-// O = sum 2^(m_i - M) O_i.  O is rescaled only where a row's maximum has grown by more than 2^8: weights up to 256 are as exact in
-// a floating type as those up to 1.
-// P overwrites the S that it was made from, so the next S of a stream is issued when its P V has completed.
+// O = sum 2^(m_i - M) O_i.  A stream has two S buffers, so that its next S is there before its P is done.  O is rescaled only where a row's
+// maximum has grown by more than 2^8: weights up to 256 are as exact in a floating type as those up to 1.
+// P lies over the first half of the S that it was made from, so the S after next is issued when its P V has completed.
 //
-// What bounds it: a tile of 16-bit keys and values of 128 heads' values is 64 KB, 1.45 us of an SM's share of 6.5 TB/s (2700 clocks); the products
-// take 1024 clocks of the tensor pipe, the 16384 powers 1024 of the MUFU pipe.  So HBM up to 128 rows, all three
-// alike at 256.
+// Two forms.  REP = 1 (33 to 128 rows): two warps share a row's tile.  REP = 4 (up to 32 rows): the rows stand in all four lane groups, each of
+// which takes a quarter of the slots, because 2^x of a warp's lanes costs the same however few of them are in use.
 //
-// 8-bit caches: TMA brings the codes, four warps turn them into 16-bit operands (exactly: int8 and e4m3 codes are numbers of
+// What bounds it, at 8 cache heads of 128 values and 32768 slots, one sequence (both launches, one after the other, caches larger than the L2):
+//   8 tokens x 32 heads, bf16   39.5 us.  A tile in steady state takes 0.6 us, which is HBM's rate (32 KB x 148 CTAs).  The other 22 us
+//                               are fixed: start and Q 5, first tile 3, end of the segment 3, join 4, two launches.
+//   64 tokens x 32 heads, bf16  64.6 us (532 TFLOP/s).  The soft-max: 0.9 us a tile, of which a third is 2^x at the MUFU pipe's rate; its
+//                               phases follow one another in a warp, and four warps a scheduler do not fill the gaps.
+//   8 tokens, int8 / e4m3       49 / 55 us: 1.2 us a tile for the conversion and the waits around it, where HBM would need 0.35.
+// Tiles of 128 slots with one S buffer a stream took 149 us for the 64 tokens above (nothing to do for a stream between its P and its next S).
+// Measured and not kept: streams that start half a tile apart and longer sleeps in the waits (no difference); converting warps for each stream
+// and one warp for all scales (8 tokens, int8: 50 -> 54 us; warps without an instruction were then the most frequent stall, so the loops of the
+// roles are kept short).
+//
+// 8-bit caches: TMA brings the codes, eight warps turn them into 16-bit operands (exactly: int8 and e4m3 codes are numbers of
 // both 16-bit types), and the scales of the rows go where they cost nothing: x = S (k_scale c) + log2 v_scale in one fused multiply-add, so that
 // P is the weight times v_scale, bounded by the same running maximum, and l = sum P / v_scale in another.
 //
-// Warps: 8 NS softmax (warp w reads the tensor memory lanes 32 (w mod 4) ..), two TMA producers, one that issues the products of each stream, and
-// for 8-bit caches four that convert.  Every wait is bounded; when one expires all roles stop waiting, the rows become NaN and tensor memory is freed.
+// Warps: 4 HF NS soft-max (warp w reads the tensor memory lanes 32 (w mod 4) ..), two TMA producers, one that issues the products of each
+// stream, and for 8-bit caches eight that convert.  Every wait is bounded; when one expires all roles stop waiting, the rows become NaN, copies
+// and products on their way are waited for and tensor memory is freed.
 #include "stx_tma.cuh"
 #include "stx_tree_attn.cuh"
 
