@@ -193,6 +193,7 @@ class LlamaSkipModel:
         self._finish_ws = torch.zeros(16, dtype=torch.uint8, device=self.device)
         self._graph = None
         self._draft_graphs = {}  # (nodes, tree, sampled) -> captured pass over a draft
+        self._temperature = torch.ones(1, dtype=torch.float32, device=self.device)  # of sampled passes
         self.trace = None  # when a list: per decode step and layer (x_pred, x_mlp, mlp_out, mask) copies, eager mode only
 
     # ------------------------------------------------------------------ pieces
@@ -380,8 +381,7 @@ class LlamaSkipModel:
                 "output_tokens_per_s": (n_new - 1) / (t2 - t1), "total_tokens_per_s": n_new / (t2 - t0)}
 
     # ------------------------------------------------------------------ several drafted tokens per pass
-    def _draft_body(self, tokens: torch.Tensor, parents: Optional[torch.Tensor], uniform: Optional[torch.Tensor],
-                    temperature: float) -> torch.Tensor:
+    def _draft_body(self, tokens: torch.Tensor, parents: Optional[torch.Tensor], uniform: Optional[torch.Tensor]) -> torch.Tensor:
         """One pass over a draft tokens [1,n] whose root is the settled token in slot pos: keeps the accepted path in the
         cache, advances pos and token, returns path, count and the next token as one int64 vector [n + 2]."""
         cfg = self.cfg
@@ -399,25 +399,24 @@ class LlamaSkipModel:
         if uniform is None:
             path, count, nxt = verify_draft(tokens, logits.argmax(-1).unsqueeze(0), parents=parents)
         else:
-            path, count, nxt = verify_draft(tokens, torch.softmax(logits / temperature, -1).unsqueeze(0), uniform=uniform, parents=parents)
+            path, count, nxt = verify_draft(tokens, torch.softmax(logits / self._temperature, -1).unsqueeze(0), uniform=uniform, parents=parents)
         if parents is not None:
             self.kv.keep(start, path, count)                                    # a chain's path lies in place already
         self.pos.add_(count)
-        self.token.copy_(nxt)
+        self.token.copy_(nxt.clamp(min=0))                                      # -1: the distribution had no weight; the caller raises
         return torch.cat([path[0], count, nxt])
 
-    def _draft_pass(self, tokens: list[int], parents: Optional[list[int]], uniform: Optional[torch.Tensor], temperature: float,
-                    use_graph: bool) -> list[int]:
+    def _draft_pass(self, tokens: list[int], parents: Optional[list[int]], uniform: Optional[torch.Tensor], use_graph: bool) -> list[int]:
         n = len(tokens)
         host = torch.tensor([tokens, parents or [0] * n], dtype=torch.long)
         if not use_graph:
             dev = host.to(self.device)
-            return self._draft_body(dev[:1], dev[1:] if parents else None, uniform, temperature).tolist()
-        key = (n, parents is not None, temperature if uniform is not None else None)
+            return self._draft_body(dev[:1], dev[1:] if parents else None, uniform).tolist()
+        key = (n, parents is not None, uniform is not None)
         if key not in self._draft_graphs:
             dev = host.to(self.device)
             u = None if uniform is None else uniform.clone()
-            args = (dev[:1], dev[1:] if parents else None, u, temperature)
+            args = (dev[:1], dev[1:] if parents else None, u)
             state = (self.pos.clone(), self.token.clone(), self.generated.clone())
             s = torch.cuda.Stream(device=self.device)
             s.wait_stream(torch.cuda.current_stream())
@@ -452,7 +451,7 @@ class LlamaSkipModel:
         cfg = self.cfg
         if cfg.draft_nodes < 1:
             raise ValueError("generate_speculative needs draft_nodes of at least 1 in the model's configuration")
-        if temperature < 0:
+        if not temperature >= 0:
             raise ValueError(f"temperature must not be negative, not {temperature}")
         draft = draft or prompt_lookup
         T = int(prompt_ids.numel())
@@ -461,13 +460,20 @@ class LlamaSkipModel:
         gen = torch.Generator(device=self.device).manual_seed(seed)
         draw = lambda n: torch.rand(1, n, generator=gen, device=self.device) if temperature > 0 else None
         tokens = prompt_ids.tolist()
+        self._temperature.fill_(temperature)
+
+        def settled(token: int) -> int:
+            if token < 0:
+                raise RuntimeError("generate_speculative: the model's distribution has no weight (logits that are not finite, or a temperature near 0)")
+            return token
+
         torch.cuda.synchronize()
         t0 = time.perf_counter()
         first = self.prefill(prompt_ids)
         if temperature > 0:                                                      # the root of a draft of one node, drawn
-            first = verify_draft(prompt_ids[-1:].view(1, 1), torch.softmax(self.logits / temperature, -1).view(1, 1, -1), uniform=draw(1))[2]
-            self.token.copy_(first)
-        tokens.append(int(first))
+            first = verify_draft(prompt_ids[-1:].view(1, 1), torch.softmax(self.logits / self._temperature, -1).view(1, 1, -1), uniform=draw(1))[2]
+            self.token.copy_(first.clamp(min=0))
+        tokens.append(settled(int(first)))
         t1 = time.perf_counter()
         passes = accepted = 0
         while len(tokens) < T + n_new:
@@ -483,8 +489,8 @@ class LlamaSkipModel:
                     raise ValueError("draft's parents must name an earlier drafted node each, or -1")
                 parents = [-1] + [p + 1 for p in parents]
             nodes = [tokens[-1]] + ids
-            got = self._draft_pass(nodes, parents, draw(len(nodes)), temperature, use_graph)
-            count, nxt = got[-2:]
+            got = self._draft_pass(nodes, parents, draw(len(nodes)), use_graph)
+            count, nxt = got[-2], settled(got[-1])
             tokens += [nodes[i] for i in got[1:count]] + [nxt]
             passes, accepted = passes + 1, accepted + count - 1
         t2 = time.perf_counter()

@@ -179,9 +179,24 @@ def test_refusals():
         m.generate_speculative(_prompt(90), 10)
     with pytest.raises(ValueError, match="temperature"):
         m.generate_speculative(_prompt(4), 4, temperature=-1.0)
+    with pytest.raises(RuntimeError, match="no weight"):  # logits / 1e-45 are infinite or NaN
+        m.generate_speculative(_prompt(4), 4, temperature=1e-45)
+    assert len(m.generate_speculative(_prompt(4), 4)["tokens"]) == 4  # and the model is usable
     for bad in (lambda t, n: [1] * (n + 1), lambda t, n: [500] * n, lambda t, n: ([1, 2], [-1, 1]), lambda t, n: ([1, 2], [-1])):
         with pytest.raises(ValueError, match="draft"):
             m.generate_speculative(_prompt(4), 8, bad)
     m.close()
     with pytest.raises(ValueError, match="draft_nodes"):
         _model(draft_nodes=65)
+
+
+def test_temperatures_share_a_graph():
+    """A temperature is an input of the captured pass: near zero it gives the greedy tokens (gaps between logits of the order 0.1)."""
+    m = _model(wstd=0.1)
+    prompt = _prompt(13)
+    want = m.generate_speculative(prompt, 16, lambda t, n: [])["tokens"].tolist()
+    hot = m.generate_speculative(prompt, 16, lambda t, n: [], temperature=5.0, seed=1)["tokens"].tolist()
+    graphs = len(m._draft_graphs)
+    cold = m.generate_speculative(prompt, 16, lambda t, n: [], temperature=1e-4, seed=1)["tokens"].tolist()
+    assert len(m._draft_graphs) == graphs and cold == want and hot != want
+    m.close()
