@@ -70,10 +70,11 @@ __device__ __forceinline__ TreeLine tree_line(const TreeArgs& a, const int* pre)
   TreeLine l;
   l.per = a.nkv * a.row_tiles;
   l.total = pre[a.n_seq] * l.per;
-  // Units of up to four tiles on average stay whole where the lengths are alike: two tiles more in a row cost 1 us, a part and its join 2 to 7 (5 tokens
-  // behind 200: 1 / 4 / 16 sequences 13.1 / 13.9 / 20.7 us in shares of two tiles, 11.2 / 11.3 / 13.3 in whole units).
+  // Units of up to eight tiles on average stay whole where the lengths are alike: shares of two tiles end inside units and need the join.  5 tokens of
+  // 24 heads on 8, 16-bit cache, shares / whole units: behind 200 slots 13.1 / 11.2 us (16 sequences 20.7 / 13.3), behind 380 18.1 / 13.3, behind 500
+  // 13.1 / 13.7 (16 sequences 24.1 / 15.1; one of int8 14.5 / 18.0).
   const int units = a.n_seq * l.per;
-  l.ctas = max(1, min(a.grid, l.total <= 4 * units ? units : l.total / a.min_tiles));
+  l.ctas = max(1, min(a.grid, l.total <= 8 * units ? units : l.total / a.min_tiles));
   l.each = l.total / l.ctas;
   l.more = l.total - l.each * l.ctas;
   return l;
