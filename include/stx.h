@@ -468,7 +468,7 @@ int stx_kv_append(const stx_kv* cache, const stx_heads* k, const stx_heads* v, i
  * for (start NULL: 0); zeros for slots outside 0..max_len-1.                                                               */
 int stx_kv_read(const stx_kv* cache, const int64_t* start, int64_t n, void* k_out, void* v_out, void* stream);
 
-/* Slot start[b] + i takes the row of slot start[b] + path[b, i], for i < counts[b], as if all rows were read before the
+/* Slot start[b] + i takes the row of slot start[b] + path[b, i], for i < counts[b] (none where it is negative), as if all rows were read before the
  * first is written; a pair with a slot outside 0..max_len-1 is skipped.  path [n_seq, n_path], row stride path_stride,
  * n_path <= STX_DRAFT_MAX.  The cache has `layers` layers, layer_stride elements (scale_layer_stride scales) apart, and all
  * of them are treated the same way in one launch.                                                                          */

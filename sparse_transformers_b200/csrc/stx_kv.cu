@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(256) k_kv_keep(unsigned char* k, unsigned char
   const int64_t l = blockIdx.z;
   pdl_wait();
   pdl_launch_dependents();
-  const int n = static_cast<int>(min(static_cast<long long>(n_path), static_cast<long long>(counts[b])));
+  // Cut to 0 .. n_path in 64 bits: below, n is compared with unsigned thread numbers too.
+  const int n = static_cast<int>(max(0ll, min(static_cast<long long>(n_path), static_cast<long long>(counts[b]))));
   const int64_t s0 = start[b];
   unsigned char* data = (blockIdx.x & 1 ? v : k) + l * layer + b * seq + h * head;
   float* scale = blockIdx.x & 1 ? vs : ks;
