@@ -3,12 +3,16 @@
 // A CTA per SM walks its segments (stx_tree_attn.cuh): up to 128 rows (tokens x query heads of a cache head) against tiles of KT = 64
 // slots.  Per tile
 //   S = Q K^T      tcgen05.mma, 128 x KT, both operands in shared memory (128-byte swizzle), S in tensor memory
-//   P = 2^(S c - m)  soft-max warps; P goes back to tensor memory in the model's type: one rounding of a weight, half a step
+//   P = 2^(S c - m)  soft-max warps; P goes back to tensor memory in the model's type: one rounding of a weight, half a step (the general kernel
+//                  holds weights in fp32, so this one's error against 64 bits is about a third larger on long contexts: 2.25e-3 for 1.65e-3 in bf16).
+//                  fp16: the base is 7 lower, so that P fills the type up to 2^15 and is subnormal only below 2^-21 of the largest weight, not 2^-14
+//                  (a slot that draws e^12 times the weight of the others and holds zeros is common, and they are all that the result consists of)
 //   O += P V       tcgen05.mma, P from tensor memory, V as it lies in the cache ([slots][head_dim] is an MN-major operand)
 // With heads of up to 128 two streams of tiles (even and odd ones of the segment) with S, O, m and l of their own share the CTA:
 // while one's soft-max runs, the other one's products do, and neither waits for the other before the segment's end, where
 // O = sum 2^(m_i - M) O_i.  A stream has two S buffers, so that its next S is there before its P is done.  O is rescaled only where a row's
-// maximum has grown by more than 2^8: weights up to 256 are as exact in a floating type as those up to 1.
+// maximum has grown by more than 2^8: weights up to 256 are as exact in a floating type as those up to 1 (a published refinement of the one-pass
+// soft-max, as is the conversion of int8 codes by way of an exponent's last places below).
 // P lies over the first half of the S that it was made from, so the S after next is issued when its P V has completed.
 //
 // Two forms.  REP = 1 (33 to 128 rows): two warps share a row's tile.  REP = 4 (up to 32 rows): the rows stand in all four lane groups, each of
@@ -27,7 +31,11 @@
 //
 // 8-bit caches: TMA brings the codes, eight warps turn them into 16-bit operands (exactly: int8 and e4m3 codes are numbers of
 // both 16-bit types), and the scales of the rows go where they cost nothing: x = S (k_scale c) + log2 v_scale in one fused multiply-add, so that
-// P is the weight times v_scale, bounded by the same running maximum, and l = sum P / v_scale in another.
+// P is the weight times v_scale, bounded by the same running maximum, and l = sum P / v_scale in another.  The maximum is of weight times scale, what a
+// row adds to O at most.  A row of zeros (scale 0) adds nothing to O: it takes the stand-in TM_ZERO_SCALE, below every scale of a row that fp16 results
+// can show (its largest value is 448 scales at most, and 2^-40 * 448 is under half of fp16's smallest number), so that it does not push the others'
+// P down, and its weight still enters l.  (Limits, bf16 only: a weight's part of l underflows next to a scale 2^100 times its row's, 2^60 for a row of
+// zeros, and l overflows where every scale is below 2^-110.)
 //
 // Warps: 4 HF NS soft-max (warp w reads the tensor memory lanes 32 (w mod 4) ..), two TMA producers, one that issues the products of each
 // stream, and for 8-bit caches eight that convert.  Every wait is bounded; when one expires all roles stop waiting, the rows become NaN, copies
@@ -43,6 +51,7 @@ namespace stx {
 
 constexpr int TM_ROWS = 128;
 constexpr float TM_SLACK = 8.f;  // in powers of two
+constexpr float TM_ZERO_SCALE = 9.094947017729282e-13f;  // 2^-40, exact in log2 and inverse
 constexpr uint32_t TM_WAIT_LIMIT = 1u << 17;  // polls of up to 4 us: half a second
 
 template <int STORE, int HD, int REP> struct TmShape {
@@ -324,6 +333,7 @@ template <typename T, int STORE, int KT, bool TAIL, int N>
 __device__ __forceinline__ float tm_row_weights(const uint32_t (&r)[N], uint32_t p_addr, const float* sc, float c, float base) {
   float l[4] = {0.f, 0.f, 0.f, 0.f};
   uint32_t p16[N / 2];
+  if constexpr (DT<T>::id == STX_F16) base -= 7.f;  // P up to 2^15 (TM_SLACK + 7); O and l carry the same factor
 #pragma unroll
   for (int j = 0; j < N; j += 4) {
     float p[4], iv[4] = {1.f, 1.f, 1.f, 1.f};
@@ -867,7 +877,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
           tm_arrive(&full[s]);
         }
         if (half == 0 && ct < KT) {
-          const float v = vs == 0.f ? 1.f : vs;  // a row of zeros: any scale
+          const float v = vs == 0.f ? TM_ZERO_SCALE : vs;
           const uint32_t ss = st * Z::SCALES + m % Z::SCALES;
           float* sc = sc_s + ss * 3 * KT;
           sc[ct] = ks * c;

@@ -33,3 +33,78 @@ def test_keep_of_no_rows_leaves_the_cache(store, none):
         for i in range(4):
             want[:, 1, :, 10 + i] = old[:, 1, :, 10 + int(block[1, i])]
         assert torch.equal(now, want)
+
+
+def weight_slack(q, layer, length, counts, masks):
+    """Elementwise bound for o = sum w_j v_j, relative to sum w_j |v_j| and not to the largest value of the cache.  A weight's relative
+    error is at most twice its score's (its own and the sum's; a score's sum of hd products as in draftref.attention_slack) + half a
+    step where it is held in 16 bits + 2^-16 for scores in powers of two of magnitude up to 64 in fp32 (2^-18 each for the product, the
+    scale's logarithm, and both again in the sum).  In fp16 a weight times its row's scale (1 for 16-bit caches, 2^-40 for a row of
+    zeros) is held as P with the largest such product at 2^7 at least: smaller than 2^-21 of it, P is a subnormal number and off
+    by 2^-25, that is by 2^-32 of the largest product, times the row's code."""
+    k, v = held_rows(layer)
+    n = layer.k.shape[2]
+    rel = ref.attention_slack(q, k, v, q.dtype) / float(v.abs().amax()) + 2.0 ** -16
+    sum_abs = ref.attention(q, k, v.abs(), length, counts, masks, n)
+    slack = rel * sum_abs
+    if q.dtype == F16:
+        s = torch.ones(layer.v.shape[:3], device=DEV).double() if layer.v_scale is None else layer.v_scale.double()
+        one = torch.eye(n, dtype=torch.float64, device=DEV).expand(*k.shape[:2], n, n)
+        wide = lambda t: torch.nn.functional.pad(t, (0, n - t.shape[-1]))  # as many values a head as there are slots
+        w = ref.attention(wide(q), wide(k), one, length, counts, masks, n, q.shape[-1] ** -0.5)  # [B,T,heads,n]
+        G = q.shape[2] // k.shape[1]
+        most = (w * torch.where(s > 0, s, 2.0 ** -40).repeat_interleave(G, 1)[:, None]).amax(-1)
+        codes = (layer.v.float().double().abs() * (s > 0)[..., None]).sum(2).repeat_interleave(G, 1)  # [B,heads,hd]
+        slack = slack + 2.0 ** -32 * most[..., None] * codes[:, None]
+    return slack
+
+
+def zero_row_case(dtype, store, hd, T, amp, lead, n=300, zero=(5, 70, 131, 250), heads=4, kv=2, seed=0):
+    """A cache whose values are of size amp, but for rows of zeros whose keys every query likes by `lead` more than the others."""
+    from sparse_transformers_b200 import KVCache
+
+    g = gen(seed)
+    base = torch.randn(hd, generator=g, device=DEV)
+    base *= hd ** 0.5 / base.norm()
+    q = (base + 0.3 * torch.randn(2, T, heads, hd, generator=g, device=DEV)).to(dtype)
+    rows = n + T
+    k = 0.5 * torch.randn(2, rows, kv, hd, generator=g, device=DEV)
+    v = amp * torch.randn(2, rows, kv, hd, generator=g, device=DEV)
+    k[:, list(zero)] = base * lead / hd ** 0.5
+    v[:, list(zero)] = 0
+    layer = KVCache(2, kv, rows, hd, dtype=dtype, store=store, device=DEV).layer(0)
+    layer.append(k.to(dtype), v.to(dtype), i64(0, 0))
+    return layer, q, i64(n, n - 65)
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, "int8"), (F16, "e4m3"), (BF16, "int8"), (BF16, "e4m3"), (F32, "int8"), (F16, "same")])
+@pytest.mark.parametrize("hd,T", [(64, 3), (128, 3), (128, 40), (256, 1), (256, 40)])
+@pytest.mark.parametrize("amp", [1.0, 0.02, 0.002])
+@pytest.mark.parametrize("lead", [0.0, 8.0, 12.0])
+def test_value_rows_of_zeros_take_no_bits_from_the_others(dtype, store, hd, T, amp, lead):
+    """A row of zeros (never written, padding, or flushed) adds to the soft-max's sum and to nothing else, whatever the other
+    rows' scales are."""
+    from sparse_transformers_b200 import tree_attention
+
+    layer, q, length = zero_row_case(dtype, store, hd, T, amp, lead, seed=hd + T)
+    k, v = held_rows(layer)
+    want = ref.attention(q, k, v, length, None, None, layer.k.shape[2])
+    assert_within(tree_attention(q, layer, length), want, half_step(want, dtype) + weight_slack(q, layer, length, None, None))
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, "int8"), (F16, "e4m3"), (BF16, "int8")])
+@pytest.mark.parametrize("T", [3, 40])
+def test_value_rows_of_very_different_sizes(dtype, store, T):
+    """Rows from 2^-14 to 1, rows of zeros first, last and a whole tile of them; a cache of nothing but zeros gives zeros."""
+    from sparse_transformers_b200 import tree_attention
+
+    layer, q, length = zero_row_case(dtype, store, 128, T, 1.0, 6.0, zero=tuple(range(64)) + (299,), seed=T)
+    g = gen(T + 1)
+    size = 2.0 ** (-14 * torch.rand(2, 2, layer.k.shape[2], generator=g, device=DEV))
+    layer.v_scale.mul_(size)
+    k, v = held_rows(layer)
+    want = ref.attention(q, k, v, length, None, None, layer.k.shape[2])
+    assert_within(tree_attention(q, layer, length), want, half_step(want, dtype) + weight_slack(q, layer, length, None, None))
+    layer.v.view(torch.uint8).zero_()
+    layer.v_scale.zero_()
+    assert bool((tree_attention(q, layer, length) == 0).all())
