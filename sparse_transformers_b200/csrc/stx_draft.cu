@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(VF_THREADS, 2) k_verify_walk(const VerifyArgs 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_launch_dependents();
-  const int n = static_cast<int>(a.counts ? min(static_cast<long long>(a.n_tok), static_cast<long long>(a.counts[b])) : a.n_tok);
+  const int n = static_cast<int>(a.counts ? max(0ll, min(static_cast<long long>(a.n_tok), static_cast<long long>(a.counts[b]))) : a.n_tok);
   const int64_t at = b * a.n_tok;
   for (int i = tid; i < a.n_tok; i += VF_THREADS) {
     x_s[i] = a.tokens[at + i];
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(32) k_verify_tokens(const VerifyArgs a, const 
   const int lane = threadIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  const int n = static_cast<int>(a.counts ? min(static_cast<long long>(a.n_tok), static_cast<long long>(a.counts[b])) : a.n_tok);
+  const int n = static_cast<int>(a.counts ? max(0ll, min(static_cast<long long>(a.n_tok), static_cast<long long>(a.counts[b]))) : a.n_tok);
   for (int i = lane; i < a.n_tok; i += 32) {
     x_s[i] = a.tokens[at + i];
     par_s[i] = a.parents ? a.parents[at + i] : i - 1;

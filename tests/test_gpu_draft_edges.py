@@ -108,3 +108,26 @@ def test_value_rows_of_very_different_sizes(dtype, store, T):
     layer.v.view(torch.uint8).zero_()
     layer.v_scale.zero_()
     assert bool((tree_attention(q, layer, length) == 0).all())
+
+
+@pytest.mark.parametrize("mode", ["greedy", "tree", "chain"])
+def test_verify_counts_far_from_the_nodes(mode):
+    """A count is a 64-bit number: far below zero nothing is in use, far above all nodes are."""
+    from sparse_transformers_b200 import verify_draft
+
+    V, T = 40, 6
+    counts = i64(-1, 0, -(1 << 32) + 3, -(1 << 63), T, T + 1, (1 << 32) + 1, (1 << 63) - 1)
+    B = counts.numel()
+    g = gen(4)
+    p = torch.softmax(torch.randn(1, T, V, generator=g, device=DEV), -1).expand(B, T, V).contiguous()
+    x, u = torch.randint(0, V, (1, T), generator=g, device=DEV).repeat(B, 1), torch.rand(1, T, generator=g, device=DEV).repeat(B, 1)
+    if mode == "greedy":
+        path, count, nxt = verify_draft(x, x.roll(-1, 1), counts=counts)
+    elif mode == "tree":
+        path, count, nxt = verify_draft(x, p, uniform=u, parents=torch.arange(-1, T - 1, device=DEV).repeat(B, 1), counts=counts)
+    else:
+        path, count, nxt = verify_draft(x, p, uniform=u, draft=p[:, 1:].contiguous(), counts=counts)
+    assert bool((path[:4] == -1).all()) and count[:4].tolist() == [0] * 4 and nxt[:4].tolist() == [-1] * 4
+    for b in range(5, B):
+        assert torch.equal(path[b], path[4]) and count[b] == count[4] and nxt[b] == nxt[4]
+    assert int(count[4]) >= 1 and int(nxt[4]) >= 0
