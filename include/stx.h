@@ -488,11 +488,16 @@ int stx_draft_masks(const int64_t* parents, int64_t n_seq, int64_t n_tokens, int
  * q, out: [n_seq, n_tokens, n_heads, head_dim] in cache->dtype; n_tokens <= STX_DRAFT_MAX, n_seq <= 1024,
  * head_dim <= 256 (a multiple of 8; of 16 for the 8-bit stores), n_heads / n_kv_heads <= 64.
  * workspace: stx_tree_attention_workspace_bytes() bytes of device memory, 16-byte aligned, in any state; it is written and
- * read by the call only, so calls that may overlap need one each.                                                          */
+ * read by the call only, so calls that may overlap need one each.
+ * Waits inside the call are bounded (environment STX_TREE_WAIT_ITERS, read by each call, default 2^17 polls, about half a
+ * second): where one expires the call ends, rows of its output are NaN, and stx_tree_attention_status says so.             */
 int stx_tree_attention_workspace_bytes(int64_t n_tokens, int n_heads, int n_kv_heads, int head_dim, int dtype, size_t* bytes_out);
 int stx_tree_attention(const stx_kv* cache, const stx_heads* q, const stx_heads* out, int64_t n_tokens, int n_heads, float scale,
                        const int64_t* length, const int64_t* counts, const int64_t* masks, int64_t mask_stride, void* workspace,
                        void* stream);
+/* SYNCHRONISES the stream; *status_out = STX_ERR_TIMEOUT when a wait of a stx_tree_attention call on the current device has expired
+ * since the last call of this entry that said so, else STX_OK.                                                             */
+int stx_tree_attention_status(int* status_out, void* stream);
 
 /* Walks a draft with the target's choices and gives the accepted nodes and the next token.
  * tokens [n_seq, n_tokens] (node i's token; tokens[b, 0] is the root's and not looked at).  Results, all int64: path

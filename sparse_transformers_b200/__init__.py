@@ -50,10 +50,10 @@ from .layer import SparseLayer, SparseStack  # noqa: E402
 from .skip import FastLoRAProjection, SkipMLP, compute_binary_mask  # noqa: E402
 from .rope import RotaryPositions, rotary_frequencies  # noqa: E402
 from .kv_cache import KVCache, KVLayer  # noqa: E402
-from .draft import draft_masks, tree_attention, verify_draft  # noqa: E402
+from .draft import attention_timed_out, draft_masks, tree_attention, verify_draft  # noqa: E402
 
 __all__ = [
     "WeightCache", "sparse_mlp_forward", "approx_topk_threshold",
     "SparseLayer", "SparseStack", "FastLoRAProjection", "SkipMLP", "compute_binary_mask",
-    "RotaryPositions", "rotary_frequencies", "KVCache", "KVLayer", "draft_masks", "tree_attention", "verify_draft",
+    "RotaryPositions", "rotary_frequencies", "KVCache", "KVLayer", "attention_timed_out", "draft_masks", "tree_attention", "verify_draft",
 ]

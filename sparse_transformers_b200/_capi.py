@@ -117,6 +117,7 @@ SIGNATURES = {
     "stx_draft_masks": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp]),
     "stx_tree_attention_workspace_bytes": (_i32, [_i64, _i32, _i32, _i32, _i32, _psz]),
     "stx_tree_attention": (_i32, [_pkv, _pheads, _pheads, _i64, _i32, _f32, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "stx_tree_attention_status": (_i32, [ctypes.POINTER(ctypes.c_int), _vp]),
     "stx_verify_draft": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
 }
 

@@ -390,4 +390,9 @@ int stx_tree_attention(const stx_kv* cache, const stx_heads* q, const stx_heads*
   });
 }
 
+int stx_tree_attention_status(int* status_out, void* stream) {
+  STX_CHECK_ARG(status_out, "stx_tree_attention_status: null pointer");
+  return tree_status(status_out, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -25,6 +25,7 @@ struct TreeArgs {
   int tile_tok, row_tiles;  // tokens of a row tile, row tiles of a (sequence, cache head)
   int min_tiles;            // fewest tiles that are worth a CTA of their own
   int grid;                 // CTAs of the first launch
+  uint32_t wait_polls;      // of a wait in the tensor-core kernel
   float* part;              // [2 grid][hd / 4][ROWS][4], then [2 grid][2][ROWS]
 };
 
@@ -142,5 +143,6 @@ int launch_tree_join(const TreeArgs& a, int rows, int kt, int dtype, cudaStream_
 // The tensor-core kernel (stx_tree_attn_mma.cu): 16-bit models, caches that a tensor map can describe.
 bool tree_mma_wanted(const stx_kv* cache);
 int tree_mma(TreeArgs a, const stx_kv* cache, cudaStream_t s);
+int tree_status(int* out, cudaStream_t s);
 
 }  // namespace stx

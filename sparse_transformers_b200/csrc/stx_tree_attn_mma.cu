@@ -39,20 +39,23 @@
 //
 // Warps: 4 HF NS soft-max (warp w reads the tensor memory lanes 32 (w mod 4) ..), two TMA producers, one that issues the products of each
 // stream, and for 8-bit caches eight that convert.  Every wait is bounded; when one expires all roles stop waiting, the rows become NaN, copies
-// and products on their way are waited for and tensor memory is freed.
+// and products on their way are waited for, tensor memory is freed, and stx_tree_attention_status reports it.
 #include "stx_tma.cuh"
 #include "stx_tree_attn.cuh"
 
 #include <cuda.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace stx {
 
 constexpr int TM_ROWS = 128;
 constexpr float TM_SLACK = 8.f;  // in powers of two
 constexpr float TM_ZERO_SCALE = 9.094947017729282e-13f;  // 2^-40, exact in log2 and inverse
-constexpr uint32_t TM_WAIT_LIMIT = 1u << 17;  // polls of up to 4 us: half a second
+constexpr uint32_t TM_WAIT_LIMIT = 1u << 17;  // polls of up to 4 us: half a second (TreeArgs::wait_polls has the limit in force)
+
+__device__ int tree_expired;  // DEV_TIMEOUT once a wait of a call on this device has expired
 
 template <int STORE, int HD, int REP> struct TmShape {
   static constexpr bool CODED = STORE != STX_STORE_SAME;
@@ -88,13 +91,18 @@ template <int STORE, int HD, int REP> struct TmShape {
   static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1 + TM_ROWS) + 64 <= 227 * 1024, "shared memory of a CTA");
 };
 
-__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-  for (uint32_t it = 0; it < TM_WAIT_LIMIT; ++it) {
+// Whether a wait of this CTA has expired, and the polls after which one does.
+struct TmDead {
+  volatile int* flag;
+  uint32_t polls;
+};
+__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, const TmDead& dead) {
+  for (uint32_t it = 0; it < dead.polls; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 63) == 63 && *dead) return false;
+    if ((it & 63) == 63 && *dead.flag) return false;
     if (it > 4096) __nanosleep(64);
   }
-  *dead = 1;
+  *dead.flag = 1;
   return false;
 }
 __device__ __forceinline__ void tm_arrive(uint64_t* bar) {
@@ -388,7 +396,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   uint64_t *k_full = bars, *k_empty = k_full + NS * DK, *v_full = k_empty + NS * DK, *v_empty = v_full + NS * DV, *s_full = v_empty + NS * DV;
   uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + NS, *raw_full = drain + NS;
   uint64_t *raw_empty = raw_full + 2 * Z::RAW, *sc_full = raw_empty + 2 * Z::RAW;  // K's, then V's
-  volatile int* dead = &dead_s;
+  const TmDead dead = {&dead_s, a.wait_polls};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (tid == 0) {
@@ -619,7 +627,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         const float mk = ml_s[HF * k * TM_ROWS + tl];
         f[k] = mk == big ? 1.f : exp2f(mk - big);
       }
-      const bool gone = !ok || *dead;
+      const bool gone = !ok || *dead.flag;
       const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
       const int slot = 2 * cta + (w.x == begin ? 0 : 1);
       float* po = tree_part_o(a, TM_ROWS, slot);
@@ -630,7 +638,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         if (!whole) {
           float* ml = tree_part_ml(a, TM_ROWS, slot);
           ml[row] = big;
-          ml[TM_ROWS + row] = sum;
+          ml[TM_ROWS + row] = gone ? inv_row : sum;  // NaN: a part of which nothing was seen would count as one that has nothing to see
         }
       }
       const unsigned long long bad = bad_s;
@@ -897,7 +905,8 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   __syncwarp();
   tm_fence_before();
   __syncthreads();
-  if (*dead) {  // a wait has expired: no copy and no product may still be on its way when the CTA leaves
+  if (*dead.flag) {  // a wait has expired: no copy and no product may still be on its way when the CTA leaves
+    if (tid == 0) atomicOr(&tree_expired, DEV_TIMEOUT);
     if (warp >= Z::SW && warp < Z::SW + 2) {
       const int half = warp - Z::SW;
       const uint32_t d = Z::CODED ? Z::RAW : half ? DV : DK;
@@ -1017,6 +1026,8 @@ int tree_mma(TreeArgs a, const stx_kv* cache, cudaStream_t s) {
   a.row_tiles = (a.n_tok + a.tile_tok - 1) / a.tile_tok;
   a.min_tiles = 2;
   a.grid = num_sms();
+  a.wait_polls = TM_WAIT_LIMIT;
+  if (const char* e = getenv("STX_TREE_WAIT_ITERS")) a.wait_polls = static_cast<uint32_t>(std::max(0ll, std::min(1ll << 22, atoll(e))));
   auto ok = [](const void* p, int64_t x, int64_t y, int64_t z) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && x % 8 == 0 && y % 8 == 0 && z % 8 == 0; };
   const int vec = ok(a.q, a.q_seq, a.q_tok, a.q_head) && ok(a.out, a.o_seq, a.o_tok, a.o_head);
   const bool few = a.tile_tok * a.group <= TM_ROWS / 4;
@@ -1028,6 +1039,19 @@ int tree_mma(TreeArgs a, const stx_kv* cache, cudaStream_t s) {
     return few ? launch_mma<T, S, 256, 4>(a, cache, o, vec, s) : launch_mma<T, S, 256, 1>(a, cache, o, vec, s);
   };
   return by_store(cache->store, [&](auto st) -> int { return cache->dtype == STX_F16 ? by_heads(__half(), st) : by_heads(__nv_bfloat16(), st); });
+}
+
+int tree_status(int* out, cudaStream_t s) {
+  int v = 0;
+  STX_CUDA(cudaMemcpyFromSymbolAsync(&v, tree_expired, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+  STX_CUDA(cudaStreamSynchronize(s));
+  *out = v & DEV_TIMEOUT ? STX_ERR_TIMEOUT : STX_OK;
+  if (v) {
+    v = 0;
+    STX_CUDA(cudaMemcpyToSymbolAsync(tree_expired, &v, sizeof(int), 0, cudaMemcpyHostToDevice, s));
+    STX_CUDA(cudaStreamSynchronize(s));
+  }
+  return STX_OK;
 }
 
 }  // namespace stx

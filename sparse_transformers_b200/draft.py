@@ -1,10 +1,12 @@
 """Decoding from drafted tokens: what the nodes of a draft see, their attention over the cache, their verification."""
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
 
+from . import _capi as C
 from .kv_cache import KVLayer
 
 _masks = torch.ops.sparse_mlp.draft_masks.default
@@ -25,8 +27,17 @@ def tree_attention(q: torch.Tensor, cache: KVLayer, length: torch.Tensor, *, tre
     length int64 [n_seq]: tokens before the draft, seen by every node; node j stands in slot length[b] + j.  tree: int64 [nodes] or
     [n_seq or 1, nodes], bit j of node i's word set when it sees node j (default: a chain, j <= i).  counts int64 [n_seq]: nodes
     in use (default all).  A node that sees nothing, or is not in use, gets zeros.  heads may be a multiple of the cache's.
-    scale: of the scores, head_dim^-1/2 by default."""
+    scale: of the scores, head_dim^-1/2 by default.  Waits inside the kernel are bounded: see attention_timed_out."""
     return _attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, length, tree, counts, scale, out)
+
+
+def attention_timed_out(device: Optional[torch.device] = None) -> bool:
+    """True when a wait inside a tree_attention call on the device (default: the current one) gave up since this function last
+    said so; rows of that call's result are NaN.  Synchronises the current stream."""
+    st = ctypes.c_int()
+    with torch.cuda.device(device):
+        C.check(C.lib.stx_tree_attention_status(ctypes.byref(st), torch.cuda.current_stream().cuda_stream))
+    return st.value != C.OK
 
 
 def verify_draft(tokens: torch.Tensor, target: torch.Tensor, *, uniform: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None,

@@ -34,7 +34,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _capi as C
-from .draft import draft_masks, tree_attention, verify_draft
+from .draft import attention_timed_out, draft_masks, tree_attention, verify_draft
 from .kv_cache import KVCache
 from .layer import SparseLayer
 from .rope import RotaryPositions
@@ -377,8 +377,14 @@ class LlamaSkipModel:
             self.decode_step(use_graph)
         torch.cuda.synchronize()
         t2 = time.perf_counter()
+        if self.cfg.kv_store != "same":
+            self._check_waits()
         return {"tokens": self.generated[:n_new].clone(), "ttft_s": t1 - t0, "decode_s": t2 - t1,
                 "output_tokens_per_s": (n_new - 1) / (t2 - t1), "total_tokens_per_s": n_new / (t2 - t0)}
+
+    def _check_waits(self) -> None:
+        if attention_timed_out(self.device):
+            raise RuntimeError("a bounded wait inside tree_attention expired: the tokens of this run are invalid")
 
     # ------------------------------------------------------------------ several drafted tokens per pass
     def _draft_body(self, tokens: torch.Tensor, parents: Optional[torch.Tensor], uniform: Optional[torch.Tensor]) -> torch.Tensor:
@@ -494,6 +500,7 @@ class LlamaSkipModel:
             tokens += [nodes[i] for i in got[1:count]] + [nxt]
             passes, accepted = passes + 1, accepted + count - 1
         t2 = time.perf_counter()
+        self._check_waits()
         new = torch.tensor(tokens[T:], dtype=torch.long, device=self.device)
         return {"tokens": new, "ttft_s": t1 - t0, "decode_s": t2 - t1, "output_tokens_per_s": (n_new - 1) / (t2 - t1),
                 "total_tokens_per_s": n_new / (t2 - t0), "passes": passes, "accepted": accepted}
