@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) k_tree_attn_any(const TreeArgs 
                                                                const KvPtr<typename Held<T, STORE>::C> vc, int vec) {
   typedef typename Held<T, STORE>::C C;
   extern __shared__ __align__(16) float tg[];
-  __shared__ int pre[TREE_MAX_SEQ + 1];
+  __shared__ int pre[TREE_PRE];
   __shared__ unsigned long long bits_s[ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hdp = (a.hd + 3) / 4 * 4, d4n = hdp / 4;
@@ -192,7 +192,7 @@ constexpr int TJ_THREADS = 256;
 // Bound by trips to memory (unit, then m and l, then the parts): about 4 us; the parts lie in the L2.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const TreeArgs a, int kt, int by_unit) {
-  __shared__ int pre[TREE_MAX_SEQ + 1];
+  __shared__ int pre[TREE_PRE];
   __shared__ float m_s[TJ_THREADS], l_s[TJ_THREADS];
   __shared__ float4 o_s[TJ_THREADS];
   tree_prefix(a, kt, pre);
@@ -379,8 +379,9 @@ int stx_tree_attention(const stx_kv* cache, const stx_heads* q, const stx_heads*
   const int rows = group * a.n_tok > 16 ? 64 : 16;  // 64 rows read a key four times less often, 16 leave fewer of them empty
   a.tile_tok = std::min(a.n_tok, rows / group);
   a.row_tiles = (a.n_tok + a.tile_tok - 1) / a.tile_tok;
-  a.min_tiles = 2;
-  a.grid = num_sms() * (rows == 16 ? 2 : 1);
+  a.sms = num_sms();
+  a.grid = a.sms * (rows == 16 ? 2 : 1);
+  a.cut = a.join = a.join_one = 0;  // a tile (11 or 22 us at 128 values) takes longer than any of them
   return by_dtype(cache->dtype, [&](auto tag) -> int {
     typedef decltype(tag) T;
     return by_store(cache->store, [&](auto st) -> int {

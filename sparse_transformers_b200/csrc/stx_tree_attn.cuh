@@ -23,8 +23,10 @@ struct TreeArgs {
   float scale_log2;  // scale * log2(e): soft-max in powers of two
   int n_seq, n_tok, nkv, group, hd;
   int tile_tok, row_tiles;  // tokens of a row tile, row tiles of a (sequence, cache head)
-  int min_tiles;            // fewest tiles that are worth a CTA of their own
-  int grid;                 // CTAs of the first launch
+  int grid;                 // CTAs of the first launch, one or two an SM
+  int sms;
+  int cut, join, join_one;  // what splitting units costs, in tiles of this kernel (tree_line): a second segment in a CTA and the join, or the
+                            // join alone; and the join of a single unit
   uint32_t wait_polls;      // of a wait in the tensor-core kernel
   float* part;              // [2 grid][hd / 4][ROWS][4], then [2 grid][2][ROWS]
 };
@@ -42,15 +44,17 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
 // A sequence without keys still has a tile: its rows are written (as zeros) by somebody.
 __device__ __forceinline__ int tree_tiles(int keys, int kt) { return keys > 0 ? (keys + kt - 1) / kt : 1; }
 
-// pre[b] = tiles of a row tile of one cache head, summed over the sequences before b; pre[n_seq] the sum.  By warp 0; the
-// caller synchronises.  The host has made sure that the whole line has less than 2^31 tiles.
+constexpr int TREE_PRE = TREE_MAX_SEQ + 2;
+// pre[b] = tiles of a row tile of one cache head, summed over the sequences before b; pre[n_seq] the sum; pre[n_seq + 1] is 1 where
+// all have the same number.  By warp 0; the caller synchronises.  The host has made sure that the whole line has less than 2^31 tiles.
 __device__ __forceinline__ void tree_prefix(const TreeArgs& a, int kt, int* pre) {
   if (threadIdx.x >= 32) return;
-  int base = 0;
+  int base = 0, most = 0, least = 0x7fffffff;
   for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
     const int b = b0 + static_cast<int>(threadIdx.x);
     const int own = b < a.n_seq ? tree_tiles(tree_seq(a, b).keys, kt) : 0;
     int sum = own;
+    if (b < a.n_seq) most = max(most, own), least = min(least, own);
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, sum, off);
@@ -59,7 +63,12 @@ __device__ __forceinline__ void tree_prefix(const TreeArgs& a, int kt, int* pre)
     if (b < a.n_seq) pre[b] = base + sum - own;
     base += __shfl_sync(0xffffffffu, sum, 31);
   }
-  if (threadIdx.x == 0) pre[a.n_seq] = base;
+  most = __reduce_max_sync(0xffffffffu, most);
+  least = __reduce_min_sync(0xffffffffu, least);
+  if (threadIdx.x == 0) {
+    pre[a.n_seq] = base;
+    pre[a.n_seq + 1] = most == least;
+  }
 }
 
 struct TreeLine {
@@ -67,15 +76,28 @@ struct TreeLine {
   int each, more;   // W / G; the first W mod G CTAs have one tile more
   int per;          // units of a sequence
 };
+// Equal shares of two tiles or more, or a CTA for each unit.  Units of one length are better left whole where a share would end inside a unit and
+// begin the next (two segments), or where the tiles saved take less than the join: nt tiles against those of a share, max(2, ceil(nt units / CTAs)),
+// and the cost in tiles.  Where lengths differ, a CTA's stretch ends inside units either way, and shares are shorter.  (Comparisons only: divisions
+// here took 1 us of both launches.)  us, whole units / shares of two, one sequence (in parentheses 16; 4 of 50 to 400 slots):
+//   tiles                                     3             4             7             8
+//   5 tokens x 24 heads on 8, 128 values
+//     16-bit cache                       10.7 / 17.8   10.8 / 12.7   12.7 / 17.5   12.9 / 12.5   (16.4 / 25.2; 32.5 / 19.0)
+//     int8 cache                         12.0 / 19.2   13.1 / 13.9   16.1 / 19.1   17.2 / 13.9   (19.0 / 27.7; 36.3 / 20.9)
+//     fp32, general kernel               39.4 / 32.4   50.4 / 29.3   77.9 / 29.4   93.7 / 29.4   (134 / 133; 63.7 / 34.9)
+//   the same of 3 heads on 1, int8       12.0 / 12.2   13.0 / 12.7   16.0 / 12.7   17.2 / 12.9   (17.9 / 14.5; 21.9 / 19.9)
+//   the same of 256 values, 16-bit       17.4 / 27.6   18.6 / 17.9   22.2 / 27.7   23.4 / 18.1   (27.9 / 42.9; 57.8 / 32.2)
 __device__ __forceinline__ TreeLine tree_line(const TreeArgs& a, const int* pre) {
   TreeLine l;
   l.per = a.nkv * a.row_tiles;
   l.total = pre[a.n_seq] * l.per;
-  // Units of up to eight tiles on average stay whole where the lengths are alike: shares of two tiles end inside units and need the join.  5 tokens of
-  // 24 heads on 8, 16-bit cache, shares / whole units: behind 200 slots 13.1 / 11.2 us (16 sequences 20.7 / 13.3), behind 380 18.1 / 13.3, behind 500
-  // 13.1 / 13.7 (16 sequences 24.1 / 15.1; one of int8 14.5 / 18.0).
-  const int units = a.n_seq * l.per;
-  l.ctas = max(1, min(a.grid, l.total <= 8 * units ? units : l.total / a.min_tiles));
+  const int units = a.n_seq * l.per, nt = pre[1];
+  l.ctas = max(1, min(a.grid, l.total >> 1));
+  if (units < a.grid && nt < 4096 && pre[a.n_seq + 1] == 1) {
+    const int cost = units == 1 ? a.join_one : (nt & 1) == 0 && l.total <= 2 * a.grid ? a.join : a.cut;
+    const int share = a.grid > a.sms && l.total > 2 * a.sms ? 4 : 2;  // two CTAs an SM take twice as long
+    if (nt <= share + cost || (nt - cost - 1) * a.sms < nt * units) l.ctas = units;
+  }
   l.each = l.total / l.ctas;
   l.more = l.total - l.each * l.ctas;
   return l;

@@ -88,7 +88,7 @@ template <int STORE, int HD, int REP> struct TmShape {
   static constexpr uint32_t SMEM_ML = 2 * HF * NS * TM_ROWS * 4;  // m of a tile, two in turn; at a segment's end its m and l
   static constexpr uint32_t BARS = 2 * NS * (DK + DV) + 2 * NB + 4 * NS + 4 * RAW + (CODED ? NS * SCALES : 0);
   static constexpr uint32_t SMEM = 1024 + SMEM_TILES + SMEM_SCALES + SMEM_ML + BARS * 8 + 64;
-  static_assert(SMEM + 4 * (TREE_MAX_SEQ + 1 + TM_ROWS) + 64 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(SMEM + 4 * (TREE_PRE + TM_ROWS) + 64 <= 227 * 1024, "shared memory of a CTA");
 };
 
 // Whether a wait of this CTA has expired, and the polls after which one does.
@@ -380,7 +380,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   typedef TmShape<STORE, HD, REP> Z;
   constexpr int KT = Z::KT, NS = Z::NS, HF = Z::HF, NB = Z::NB, DK = Z::DK, DV = Z::DV;
   extern __shared__ unsigned char tm_raw[];
-  __shared__ int pre[TREE_MAX_SEQ + 1];
+  __shared__ int pre[TREE_PRE];
   __shared__ unsigned long long bad_s;  // nodes of the segment with a value that is not finite
   __shared__ uint32_t tmem_s;
   __shared__ float inv_s[TM_ROWS];
@@ -1024,13 +1024,20 @@ int tree_mma(TreeArgs a, const stx_kv* cache, cudaStream_t s) {
   if (!tm_order(cache, &o)) return STX_ERR_UNSUPPORTED;
   a.tile_tok = std::min(a.n_tok, TM_ROWS / a.group);
   a.row_tiles = (a.n_tok + a.tile_tok - 1) / a.tile_tok;
-  a.min_tiles = 2;
-  a.grid = num_sms();
+  a.grid = a.sms = num_sms();
   a.wait_polls = TM_WAIT_LIMIT;
   if (const char* e = getenv("STX_TREE_WAIT_ITERS")) a.wait_polls = static_cast<uint32_t>(std::max(0ll, std::min(1ll << 22, atoll(e))));
   auto ok = [](const void* p, int64_t x, int64_t y, int64_t z) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && x % 8 == 0 && y % 8 == 0 && z % 8 == 0; };
   const int vec = ok(a.q, a.q_seq, a.q_tok, a.q_head) && ok(a.out, a.o_seq, a.o_tok, a.o_head);
   const bool few = a.tile_tok * a.group <= TM_ROWS / 4;
+  // For tree_line, in ns and from runs over 2 to 8 tiles: a tile, a second segment in a CTA, the join.
+  const bool coded = cache->store != STX_STORE_SAME;
+  const int tile = (a.hd <= 64 ? (coded ? 900 : 400) : a.hd <= 128 ? (coded ? 1100 : 500) : coded ? 1500 : 1200) + (few ? 0 : 200);
+  const int cut = a.hd <= 64 ? 3500 : a.hd <= 128 ? 5000 : 9000;
+  const int join = few ? (a.hd <= 64 ? 2200 : a.hd <= 128 ? 2600 : 2000) : a.hd <= 64 ? 4000 : a.hd <= 128 ? 4500 : 8500;
+  a.cut = (cut + join) / tile;
+  a.join = join / tile;
+  a.join_one = join / (2 * tile);
   auto by_heads = [&](auto t, auto st) -> int {
     typedef decltype(t) T;
     constexpr int S = decltype(st)::value;

@@ -171,3 +171,18 @@ def test_a_host_run_with_expired_waits_is_refused(monkeypatch):
     monkeypatch.delenv("STX_TREE_WAIT_ITERS")
     assert m.generate_speculative(_prompt(9), 6, use_graph=False)["tokens"].tolist() == want
     m.close()
+
+
+@pytest.mark.parametrize("dtype,store,hd", [(F16, "same", 64), (BF16, "int8", 128), (F16, "e4m3", 128), (BF16, "same", 256), (F32, "same", 128)])
+@pytest.mark.parametrize("n_seq,heads,kv,T", [(1, 3, 1, 5), (1, 24, 8, 5), (3, 8, 8, 1), (18, 8, 8, 2), (37, 4, 4, 1), (3, 8, 2, 40)])
+def test_units_left_whole_and_split(dtype, store, hd, n_seq, heads, kv, T):
+    """Contexts of one to ten tiles of 64 slots, alike and one apart: units that a CTA has for itself, shares of two tiles that end with
+    units or inside them, and as many units as CTAs; the same bits on a second call."""
+    from sparse_transformers_b200 import tree_attention
+    from test_gpu_draft import attn_case, check_attention
+
+    for tiles in (1, 2, 3, 4, 5, 8, 10) if n_seq < 10 else (2, 3, 7):
+        for last in (0, 70):
+            lengths = [64 * tiles - T] * (n_seq - 1) + [max(0, 64 * tiles - T - last)]
+            case = attn_case(dtype, store, hd, heads, kv, T, lengths, tree="chain", seed=tiles)
+            assert torch.equal(check_attention(*case), tree_attention(case[1], case[0], case[2]))
