@@ -65,14 +65,16 @@ class _Rotate(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, positions, plan, inverse):
-        ctx.positions, ctx.plan, ctx.inverse = positions, plan, inverse
+        ctx.save_for_backward(positions)  # often a counter that the caller advances in place: autograd refuses it then
+        ctx.plan, ctx.inverse = plan, inverse
         with torch.no_grad():
             return _rope(x, positions, plan.turns, plan.interleaved, plan.factor, inverse, None)
 
     @staticmethod
     def backward(ctx, g):
+        (positions,) = ctx.saved_tensors
         g = g if g.stride(-1) == 1 else g.contiguous()
-        return _Rotate.apply(g, ctx.positions, ctx.plan, not ctx.inverse), None, None, None
+        return _Rotate.apply(g, positions, ctx.plan, not ctx.inverse), None, None, None
 
 
 class RotaryPositions:

@@ -186,3 +186,25 @@ def test_units_left_whole_and_split(dtype, store, hd, n_seq, heads, kv, T):
             lengths = [64 * tiles - T] * (n_seq - 1) + [max(0, 64 * tiles - T - last)]
             case = attn_case(dtype, store, hd, heads, kv, T, lengths, tree="chain", seed=tiles)
             assert torch.equal(check_attention(*case), tree_attention(case[1], case[0], case[2]))
+
+
+def test_positions_changed_before_the_gradient_are_refused():
+    """The gradient turns back by the angles of the forward pass: positions that have moved on since are an error, not other angles."""
+    from sparse_transformers_b200 import RotaryPositions
+
+    plan = RotaryPositions(32, device=DEV)
+    x = torch.randn(5, 2, 32, generator=gen(1), device=DEV).requires_grad_()
+    pos = torch.arange(5, device=DEV)
+    y = plan.rotate(x, pos)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = plan.rotate(x, pos)
+    (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    assert_within(dx.detach(), 2 * x.detach().double(), 12 * 3.1 * 2.0 ** -24 * ref.rotate_slack(x.detach(), 16, 1.0, False))  # two rotations of 3.1 2^-24 each way, doubled
+    (ddx,) = torch.autograd.grad((dx * x.detach()).sum(), x)
+    assert ddx.shape == x.shape
+    y = plan.rotate(x, pos)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
