@@ -10,6 +10,13 @@ from typing import Optional
 
 import torch
 
+# What a scaling must and may say.  original_max_position_embeddings does not matter to linear and ntk, which configurations give it all the same.
+_NEEDS = {"none": (), "linear": ("factor",), "ntk": ("factor",),
+          "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+          "yarn": ("factor", "original_max_position_embeddings")}
+_MAY = {"linear": ("original_max_position_embeddings",), "ntk": ("original_max_position_embeddings",),
+        "yarn": ("beta_fast", "beta_slow", "attention_factor")}
+
 _rope = torch.ops.sparse_mlp.rope.default
 
 
@@ -22,14 +29,27 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
       llama3   pairs that turn less than low_freq_factor times within original_max_position_embeddings are slowed by factor,
                those that turn more than high_freq_factor times are left alone, between them a linear blend
       yarn     the same idea, blended linearly over the pair's index between the pairs that turn beta_fast (32) and beta_slow (1)
-               times; the result is multiplied by attention_factor (default 0.1 ln(factor) + 1)"""
+               times; the result is multiplied by attention_factor (default 0.1 ln(factor) + 1)
+    A key that is not known to the rope_type (yarn's mscale, mscale_all_dim and truncate=False among them) is an error: it would
+    mean another rotation than this one."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be positive and even, not {rotary_dim}")
     if not theta > 0:
         raise ValueError(f"theta must be positive, not {theta}")
-    kind = "none" if scaling is None else scaling.get("rope_type", scaling.get("type", "none"))
-    if kind in ("none", "default"):
-        scaling, kind = {}, "none"
+    scaling = dict(scaling or {})
+    kind = scaling.pop("rope_type", scaling.pop("type", "none"))
+    scaling.pop("type", None)
+    kind = "none" if kind == "default" else kind
+    if kind not in _NEEDS:
+        raise ValueError(f"unknown rope_type {kind!r} (linear, ntk, llama3, yarn)")
+    if kind == "yarn" and scaling.get("truncate") is True:  # the default
+        del scaling["truncate"]
+    for key in _NEEDS[kind]:
+        if scaling.get(key) is None:
+            raise ValueError(f"rope_type {kind!r} needs {key}")
+    for key in scaling:
+        if key not in _NEEDS[kind] + _MAY.get(kind, ()):
+            raise ValueError(f"rope_type {kind!r} does not know {key}")
     factor = float(scaling.get("factor", 1.0))
     if not factor > 0:
         raise ValueError(f"factor must be positive, not {factor}")
@@ -40,20 +60,20 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
         return w, 1.0
     if kind == "linear":
         return [x / factor for x in w], 1.0
-    if kind not in ("llama3", "yarn"):
-        raise ValueError(f"unknown rope_type {kind!r} (linear, ntk, llama3, yarn)")
-    if "original_max_position_embeddings" not in scaling:
-        raise ValueError(f"rope_type {kind!r} needs original_max_position_embeddings")
     orig = float(scaling["original_max_position_embeddings"])
+    if not orig > 0:
+        raise ValueError(f"original_max_position_embeddings must be positive, not {orig}")
     if kind == "llama3":
         lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
         if not hi > lo:
             raise ValueError("high_freq_factor must be above low_freq_factor")
         keep = [min(1.0, max(0.0, (orig * x / (2 * math.pi) - lo) / (hi - lo))) for x in w]
         return [x * (k + (1.0 - k) / factor) for x, k in zip(w, keep)], 1.0
+    if not theta > 1:
+        raise ValueError(f"rope_type 'yarn' needs theta above 1, not {theta}")
     index = lambda turns: rotary_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta))
-    lo = max(math.floor(index(float(scaling.get("beta_fast", 32.0)))), 0)
-    hi = min(math.ceil(index(float(scaling.get("beta_slow", 1.0)))), rotary_dim - 1)
+    lo = max(math.floor(index(float(scaling.get("beta_fast") or 32.0))), 0)
+    hi = min(math.ceil(index(float(scaling.get("beta_slow") or 1.0))), rotary_dim - 1)
     slow = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(rotary_dim // 2)]
     given = scaling.get("attention_factor")
     return ([x * (1.0 - s + s / factor) for x, s in zip(w, slow)],

@@ -140,3 +140,34 @@ def test_prompt_lookup():
     assert prompt_lookup([7], 3) == [] and prompt_lookup([], 3) == []
     assert prompt_lookup([8, 1, 5, 8, 2, 6, 8], 1) == [2]             # the latest occurrence
     assert prompt_lookup([8, 8], 4) == [8]
+
+
+@pytest.mark.parametrize("scaling,text", [
+    (dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096, mscale=1.0, mscale_all_dim=0.8), "mscale"),
+    (dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096, truncate=False), "truncate"),
+    (dict(rope_type="linear", factor=4.0, rope_theta=5e5), "rope_theta"), (dict(rope_type="default", factor=4.0), "factor"),
+    (dict(factor=4.0), "factor"), (dict(rope_type="linear"), "needs factor"), (dict(rope_type="ntk"), "needs factor"),
+    (dict(rope_type="yarn", original_max_position_embeddings=4096), "needs factor"),
+    (dict(rope_type="llama3", factor=8.0, high_freq_factor=4.0, original_max_position_embeddings=8192), "needs low_freq_factor"),
+    (dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, original_max_position_embeddings=8192), "needs high_freq_factor"),
+    (dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0), "needs original_max_position_embeddings"),
+    (dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=0), "must be positive"), (dict(rope_type="longrope", factor=4.0), "unknown")])
+def test_rotary_scalings_that_would_be_taken_for_others_are_refused(scaling, text):
+    """A key that changes the result and is not known, or one that is missing, is an error and not another rotation."""
+    from sparse_transformers_b200 import rotary_frequencies
+
+    with pytest.raises(ValueError, match=text):
+        rotary_frequencies(64, 10000.0, scaling)
+    if scaling.get("rope_type") == "yarn":  # the pairs' places are counted in logarithms of theta
+        with pytest.raises(ValueError, match="theta"):
+            rotary_frequencies(64, 1.0, dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096))
+
+
+def test_rotary_scalings_as_configurations_spell_them():
+    from sparse_transformers_b200 import rotary_frequencies
+
+    yarn = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096)
+    assert rotary_frequencies(64, 1e4, dict(yarn, type="yarn", beta_fast=32, beta_slow=1, attention_factor=None, truncate=True)) == rotary_frequencies(64, 1e4, yarn)
+    assert rotary_frequencies(64, 1e4, dict(yarn, beta_fast=None, beta_slow=None)) == rotary_frequencies(64, 1e4, yarn)
+    assert rotary_frequencies(64, 1e4, dict(type="linear", factor=2, original_max_position_embeddings=4096)) == rotary_frequencies(64, 1e4, dict(rope_type="linear", factor=2.0))
+    assert rotary_frequencies(64, 1e4, dict(rope_type="default")) == rotary_frequencies(64, 1e4) == rotary_frequencies(64, 1e4, {})
