@@ -177,7 +177,10 @@ class LlamaSkipModel:
                                       lazy_cache=cfg.lazy_cache)
             self.layers.append(L)
         self.rope = RotaryPositions(hd, theta=cfg.rope_theta, scaling=cfg.rope_scaling, device=self.device)
-        self.cos, self.sin = rope_tables(cfg, self.device) if cfg.rope_scaling is None else self.rope.tables(cfg.max_len)
+        # One rotation a model: where keys are also rotated as they are appended, with angles formed in fp64, the tables hold those too (fp32
+        # angles are off by 5e-4 radians at position 8192).
+        plain = cfg.rope_scaling is None and cfg.draft_nodes == 0 and cfg.kv_store == "same"
+        self.cos, self.sin = rope_tables(cfg, self.device) if plain else self.rope.tables(cfg.max_len)
         self.kv = KVCache(1, cfg.kv_heads, cfg.max_len, hd, dtype=dt, store=cfg.kv_store, layers=cfg.layers, device=self.device)
         self.k_cache, self.v_cache = self.kv.k[:, 0], self.kv.v[:, 0]  # [layers, kv_heads, max_len, head_dim]
         # decode state, all on the device so that the captured step needs no host input

@@ -208,3 +208,37 @@ def test_positions_changed_before_the_gradient_are_refused():
     pos.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def first_layer_keys(m, ids):
+    """Keys of the first decoder layer before their rotation, as prefill forms them: [T, kv_heads, head_dim]."""
+    from sparse_transformers_b200.llama_skip import rms_norm
+
+    c, L = m.cfg, m.layers[0]
+    x = rms_norm(m.embed.index_select(0, ids), L["ln1"], c.rms_eps)
+    return (x @ L["wqkv"].t())[:, c.heads * c.head_dim:(c.heads + c.kv_heads) * c.head_dim].unflatten(-1, (c.kv_heads, c.head_dim))
+
+
+@pytest.mark.parametrize("draft_nodes", [0, 4])
+def test_a_model_has_one_rotation(draft_nodes):
+    """Far from the start the prompt's keys and those of drafted tokens stand at the same angles.  A table's sine and cosine are rounded once,
+    products and sum as in a rotation.  A model that neither drafts nor holds 8 bits keeps the tables that it had."""
+    from sparse_transformers_b200.llama_skip import rope_tables
+    from test_gpu_draft import TURN
+    from test_gpu_speculative import _model, _prompt
+
+    T = 8200
+    m = _model(max_len=T + 8, layers=1, draft_nodes=draft_nodes)
+    if not draft_nodes:
+        assert all(torch.equal(a, b) for a, b in zip((m.cos, m.sin), rope_tables(m.cfg, DEV)))
+        m.close()
+        return
+    ids = _prompt(T)
+    m.prefill(ids)
+    k, pos = first_layer_keys(m, ids), torch.arange(T, device=DEV)
+    want = ref.rotate(k, pos, m.rope.frequencies, 1.0, False)
+    slack = half_step(want, F32) + TURN * ref.rotate_slack(k, 32, 1.0, False)
+    assert_within(m.k_cache[0, :, :T].transpose(0, 1), want, slack, "prompt")
+    m.kv.layer(0).append(k.unsqueeze(0), k.unsqueeze(0), i64(0), rope=m.rope)
+    assert_within(m.k_cache[0, :, :T].transpose(0, 1), want, slack, "appended")
+    m.close()
