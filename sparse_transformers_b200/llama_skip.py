@@ -220,14 +220,14 @@ class LlamaSkipModel:
             o = F.scaled_dot_product_attention(q.unsqueeze(0), self.k_cache[li].unsqueeze(0), self.v_cache[li].unsqueeze(0),
                                                attn_mask=mask, enable_gqa=True)
         else:
+            if cfg.kv_store != "same":                                           # codes from the rotation's fp32 result: rounded once
+                start = torch.full((1,), pos0, dtype=torch.long, device=self.device)
+                self.kv.layer(li).append(k.transpose(0, 1).unsqueeze(0), v.transpose(0, 1).unsqueeze(0), start, rope=self.rope)
             cos, sin = self.cos[pos0:pos0 + T], self.sin[pos0:pos0 + T]
             q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
-            if cfg.kv_store == "same":
+            if cfg.kv_store == "same":                                           # (8 bits: the prompt attends to its own exact rows)
                 self.k_cache[li, :, pos0:pos0 + T] = k
                 self.v_cache[li, :, pos0:pos0 + T] = v
-            else:                                                                # the prompt attends to its own exact rows
-                start = torch.full((1,), pos0, dtype=torch.long, device=self.device)
-                self.kv.layer(li).append(k.transpose(0, 1).unsqueeze(0), v.transpose(0, 1).unsqueeze(0), start)
             o = F.scaled_dot_product_attention(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), is_causal=True, enable_gqa=True)
         o = o.squeeze(0).transpose(0, 1).reshape(T, nh * hd)
         return o @ L["wo"].t()

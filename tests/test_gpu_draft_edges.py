@@ -242,3 +242,18 @@ def test_a_model_has_one_rotation(draft_nodes):
     m.kv.layer(0).append(k.unsqueeze(0), k.unsqueeze(0), i64(0), rope=m.rope)
     assert_within(m.k_cache[0, :, :T].transpose(0, 1), want, slack, "appended")
     m.close()
+
+
+@pytest.mark.parametrize("dtype,store", [(BF16, "int8"), (F16, "e4m3"), (F16, "int8")])
+def test_a_prompts_keys_are_rounded_once(dtype, store):
+    """An 8-bit cache holds the same codes of a key whether it came with the prompt or with a draft."""
+    from test_gpu_speculative import _model, _prompt
+
+    m = _model(dtype=dtype, kv_store=store, layers=1)
+    ids = _prompt(70)
+    m.prefill(ids)
+    k = first_layer_keys(m, ids)
+    codes, scales = m.kv.k.view(torch.uint8).clone(), m.kv.k_scale.clone()
+    m.kv.layer(0).append(k.unsqueeze(0), k.unsqueeze(0), i64(0), rope=m.rope)
+    assert torch.equal(m.kv.k.view(torch.uint8), codes) and torch.equal(m.kv.k_scale, scales)
+    m.close()
