@@ -46,6 +46,13 @@ static void no_grad(const Tensor& t, const char* who, const char* name) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), who, ": has no gradient, but ", name,
               " requires one (call it under torch.no_grad())");
 }
+// The caller's tensor has been written: what autograd saved of it is stale.
+static void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+static void written(const MaybeTensor& t) {
+  if (t) written(*t);
+}
 // int64 of exactly this shape, rows contiguous; returns the row stride (0 for a single row or an expanded one).
 static int64_t index_rows(const c10::Device& d, const Tensor& t, at::IntArrayRef shape, const char* who, const char* name) {
   on(d, t, who, name);
@@ -125,7 +132,7 @@ static stx_rotary rotary_of(const c10::Device& d, const Tensor& turns, bool inte
 }
 
 // x [n, heads, hd] or [b, t, heads, hd], positions x.shape[:-2]
-Tensor rope(const Tensor& x, const Tensor& positions, const Tensor& turns, bool interleaved, double factor, bool inverse, const MaybeTensor& out) {
+static Tensor rope(const Tensor& x, const Tensor& positions, const Tensor& turns, bool interleaved, double factor, bool inverse, const MaybeTensor& out) {
   constexpr const char* who = "rope";
   on_cuda(x, who, "x");
   no_grad(x, who, "x");
@@ -148,10 +155,17 @@ Tensor rope(const Tensor& x, const Tensor& positions, const Tensor& turns, bool 
   ok(stx_rope(&hx, &hy, x4.size(0), x4.size(1), static_cast<int>(x4.size(2)), static_cast<int>(x4.size(3)), positions.data_ptr<int64_t>(), pstride,
               &rot, inverse, dt, stream_of(x.device())),
      who);
+  if (out) written(*out);
   return y;
 }
+static Tensor rope_new(const Tensor& x, const Tensor& positions, const Tensor& turns, bool interleaved, double factor, bool inverse) {
+  return rope(x, positions, turns, interleaved, factor, inverse, MaybeTensor());
+}
+static Tensor rope_out(const Tensor& x, const Tensor& positions, const Tensor& turns, bool interleaved, double factor, bool inverse, const Tensor& out) {
+  return rope(x, positions, turns, interleaved, factor, inverse, out);
+}
 
-MaybeTensor kv_append(const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs, const Tensor& k, const Tensor& v,
+static MaybeTensor kv_append(const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs, const Tensor& k, const Tensor& v,
                       const Tensor& start, const MaybeTensor& counts, const MaybeTensor& turns, bool interleaved, double factor,
                       const MaybeTensor& positions, const MaybeTensor& q, const MaybeTensor& q_out) {
   constexpr const char* who = "kv_append";
@@ -199,7 +213,18 @@ MaybeTensor kv_append(const Tensor& kc, const Tensor& vc, const MaybeTensor& ks,
   ok(stx_kv_append(&c, &hk, &hv, T, st, cn, turns ? &rot : nullptr, positions ? positions->data_ptr<int64_t>() : nullptr, pstride,
                    q ? &hq : nullptr, q ? &ho : nullptr, nh, stream_of(d)),
      who);
+  written(kc), written(vc), written(ks), written(vs), written(q_out);
   return y;
+}
+static MaybeTensor kv_append_new(const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs, const Tensor& k, const Tensor& v,
+                                 const Tensor& start, const MaybeTensor& counts, const MaybeTensor& turns, bool interleaved, double factor,
+                                 const MaybeTensor& positions, const MaybeTensor& q) {
+  return kv_append(kc, vc, ks, vs, k, v, start, counts, turns, interleaved, factor, positions, q, MaybeTensor());
+}
+static Tensor kv_append_out(const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs, const Tensor& k, const Tensor& v,
+                            const Tensor& start, const MaybeTensor& counts, const MaybeTensor& turns, bool interleaved, double factor,
+                            const MaybeTensor& positions, const MaybeTensor& q, const Tensor& q_out) {
+  return *kv_append(kc, vc, ks, vs, k, v, start, counts, turns, interleaved, factor, positions, q, q_out);
 }
 
 // dtype: stx_dtype of the values
@@ -232,6 +257,7 @@ void kv_keep(const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const Ma
   ok(stx_kv_keep(&c, kc.size(0), kc.size(0) > 1 ? kc.stride(0) : 0, ks && kc.size(0) > 1 ? ks->stride(0) : 0, index_of(d, start, c.n_seq, who, "start"),
                  path.data_ptr<int64_t>(), pstride, path.size(1), index_of(d, counts, c.n_seq, who, "counts"), stream_of(d)),
      who);
+  written(kc), written(vc), written(ks), written(vs);
 }
 
 std::tuple<Tensor, Tensor> draft_masks(const Tensor& parents) {
@@ -246,7 +272,7 @@ std::tuple<Tensor, Tensor> draft_masks(const Tensor& parents) {
 }
 
 // masks [n_tokens] or [n_seq or 1, n_tokens]
-Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs, const Tensor& length,
+static Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs, const Tensor& length,
                       const MaybeTensor& masks, const MaybeTensor& counts, std::optional<double> scale, const MaybeTensor& out) {
   constexpr const char* who = "tree_attention";
   on_cuda(q, who, "q");
@@ -282,7 +308,17 @@ Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const
   ok(stx_tree_attention(&c, &hq, &ho, T, nh, static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(c.head_dim))), ln, cn,
                         masks ? masks->data_ptr<int64_t>() : nullptr, mstride, ws.data_ptr(), stream_of(d)),
      who);
+  written(out);
   return y;
+}
+static Tensor tree_attention_new(const Tensor& q, const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs,
+                                 const Tensor& length, const MaybeTensor& masks, const MaybeTensor& counts, std::optional<double> scale) {
+  return tree_attention(q, kc, vc, ks, vs, length, masks, counts, scale, MaybeTensor());
+}
+static Tensor tree_attention_out(const Tensor& q, const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const MaybeTensor& vs,
+                                 const Tensor& length, const MaybeTensor& masks, const MaybeTensor& counts, std::optional<double> scale,
+                                 const Tensor& out) {
+  return tree_attention(q, kc, vc, ks, vs, length, masks, counts, scale, out);
 }
 
 std::tuple<Tensor, Tensor, Tensor> verify_draft(const Tensor& tokens, const Tensor& target, const MaybeTensor& uniform, const MaybeTensor& parents,
@@ -334,12 +370,20 @@ std::tuple<Tensor, Tensor, Tensor> verify_draft(const Tensor& tokens, const Tens
 
 }  // namespace stxb
 
+// The schemas name what is written, so that nobody who looks at a program by them drops or reorders these calls.
+#define STX_CACHE "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, "
+#define STX_ROPE "Tensor x, Tensor positions, Tensor turns, bool interleaved, float factor, bool inverse"
+#define STX_APPEND STX_CACHE "Tensor k, Tensor v, Tensor start, Tensor? counts, Tensor? turns, bool interleaved, float factor, Tensor? positions, Tensor? q"
+#define STX_ATTEND "Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_scale, Tensor? v_scale, Tensor length, Tensor? masks, Tensor? counts, float? scale"
 TORCH_LIBRARY_FRAGMENT(sparse_mlp, m) {
-  m.def("rope", stxb::rope);
-  m.def("kv_append", stxb::kv_append);
+  m.def("rope(" STX_ROPE ") -> Tensor", stxb::rope_new);
+  m.def("rope.out(" STX_ROPE ", *, Tensor(a!) out) -> Tensor(a!)", stxb::rope_out);
+  m.def("kv_append(" STX_APPEND ") -> Tensor?", stxb::kv_append_new);
+  m.def("kv_append.out(" STX_APPEND ", *, Tensor(e!) q_out) -> Tensor(e!)", stxb::kv_append_out);
   m.def("kv_read", stxb::kv_read);
-  m.def("kv_keep", stxb::kv_keep);
+  m.def("kv_keep(" STX_CACHE "int dtype, Tensor start, Tensor path, Tensor counts) -> ()", stxb::kv_keep);
   m.def("draft_masks", stxb::draft_masks);
-  m.def("tree_attention", stxb::tree_attention);
+  m.def("tree_attention(" STX_ATTEND ") -> Tensor", stxb::tree_attention_new);
+  m.def("tree_attention.out(" STX_ATTEND ", *, Tensor(a!) out) -> Tensor(a!)", stxb::tree_attention_out);
   m.def("verify_draft", stxb::verify_draft);
 }

@@ -11,6 +11,7 @@ from .kv_cache import KVLayer
 
 _masks = torch.ops.sparse_mlp.draft_masks.default
 _attention = torch.ops.sparse_mlp.tree_attention.default
+_attention_out = torch.ops.sparse_mlp.tree_attention.out
 _verify = torch.ops.sparse_mlp.verify_draft.default
 
 
@@ -28,7 +29,9 @@ def tree_attention(q: torch.Tensor, cache: KVLayer, length: torch.Tensor, *, tre
     [n_seq or 1, nodes], bit j of node i's word set when it sees node j (default: a chain, j <= i).  counts int64 [n_seq]: nodes
     in use (default all).  A node that sees nothing, or is not in use, gets zeros.  heads may be a multiple of the cache's.
     scale: of the scores, head_dim^-1/2 by default.  Waits inside the kernel are bounded: see attention_timed_out."""
-    return _attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, length, tree, counts, scale, out)
+    if out is None:
+        return _attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, length, tree, counts, scale)
+    return _attention_out(q, cache.k, cache.v, cache.k_scale, cache.v_scale, length, tree, counts, scale, out=out)
 
 
 def attention_timed_out(device: Optional[torch.device] = None) -> bool:

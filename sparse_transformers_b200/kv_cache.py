@@ -9,6 +9,7 @@ from . import _capi as C
 from .rope import RotaryPositions
 
 _append = torch.ops.sparse_mlp.kv_append.default
+_append_out = torch.ops.sparse_mlp.kv_append.out
 _read = torch.ops.sparse_mlp.kv_read.default
 _keep = torch.ops.sparse_mlp.kv_keep.default
 _DT = {torch.float32: C.F32, torch.float16: C.F16, torch.bfloat16: C.BF16}
@@ -31,9 +32,9 @@ class KVLayer:
         counts[b] are left as they were."""
         if rope is not None and rope.head_dim != k.shape[-1]:
             raise RuntimeError(f"kv_append: heads of {k.shape[-1]} values, the rotary plan has {rope.head_dim}")
-        if rope is None:
-            return _append(self.k, self.v, self.k_scale, self.v_scale, k, v, start, counts, None, False, 1.0, positions, q, q_out)
-        return _append(self.k, self.v, self.k_scale, self.v_scale, k, v, start, counts, rope.turns, rope.interleaved, rope.factor, positions, q, q_out)
+        plan = (None, False, 1.0) if rope is None else (rope.turns, rope.interleaved, rope.factor)
+        args = (self.k, self.v, self.k_scale, self.v_scale, k, v, start, counts, *plan, positions, q)
+        return _append(*args) if q_out is None else _append_out(*args, q_out=q_out)
 
     def read(self, start: Optional[torch.Tensor], n: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(k, v) [n_seq, kv_heads, n, head_dim] in the model's dtype: what slots start[b] .. start[b] + n - 1 stand for

@@ -18,6 +18,7 @@ _MAY = {"linear": ("original_max_position_embeddings",), "ntk": ("original_max_p
         "yarn": ("beta_fast", "beta_slow", "attention_factor")}
 
 _rope = torch.ops.sparse_mlp.rope.default
+_rope_out = torch.ops.sparse_mlp.rope.out
 
 
 def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[dict] = None) -> tuple[list[float], float]:
@@ -88,7 +89,7 @@ class _Rotate(torch.autograd.Function):
         ctx.save_for_backward(positions)  # often a counter that the caller advances in place: autograd refuses it then
         ctx.plan, ctx.inverse = plan, inverse
         with torch.no_grad():
-            return _rope(x, positions, plan.turns, plan.interleaved, plan.factor, inverse, None)
+            return _rope(x, positions, plan.turns, plan.interleaved, plan.factor, inverse)
 
     @staticmethod
     def backward(ctx, g):
@@ -123,7 +124,9 @@ class RotaryPositions:
             raise RuntimeError(f"rope: heads of {x.shape[-1]} values, the plan has {self.head_dim}")
         if x.requires_grad and torch.is_grad_enabled() and out is None:
             return _Rotate.apply(x, positions, self, inverse)
-        return _rope(x, positions, self.turns, self.interleaved, self.factor, inverse, out)
+        if out is None:
+            return _rope(x, positions, self.turns, self.interleaved, self.factor, inverse)
+        return _rope_out(x, positions, self.turns, self.interleaved, self.factor, inverse, out=out)
 
     def tables(self, max_len: int) -> tuple[torch.Tensor, torch.Tensor]:
         """cos and sin [max_len, head_dim] in fp32 for stx_attn_decode, which rotates whole heads in the half layout."""

@@ -171,3 +171,24 @@ def test_rotary_scalings_as_configurations_spell_them():
     assert rotary_frequencies(64, 1e4, dict(yarn, beta_fast=None, beta_slow=None)) == rotary_frequencies(64, 1e4, yarn)
     assert rotary_frequencies(64, 1e4, dict(type="linear", factor=2, original_max_position_embeddings=4096)) == rotary_frequencies(64, 1e4, dict(rope_type="linear", factor=2.0))
     assert rotary_frequencies(64, 1e4, dict(rope_type="default")) == rotary_frequencies(64, 1e4) == rotary_frequencies(64, 1e4, {})
+
+
+def test_written_tensors_are_named_in_the_schemas():
+    """A program that is cleaned up by its operators' schemas keeps the calls that only write."""
+    import sparse_transformers_b200  # noqa: F401
+
+    ops = torch.ops.sparse_mlp
+    writes = lambda op: [a.name for a in op._schema.arguments if a.alias_info is not None and a.alias_info.is_write]
+    cache = ["k_cache", "v_cache", "k_scale", "v_scale"]
+    assert writes(ops.kv_append.default) == cache and writes(ops.kv_keep.default) == cache and writes(ops.kv_append.out) == cache + ["q_out"]
+    assert writes(ops.rope.out) == ["out"] and writes(ops.tree_attention.out) == ["out"]
+    assert not writes(ops.rope.default) and not writes(ops.tree_attention.default) and not writes(ops.kv_read.default)
+    g = torch.fx.Graph()
+    k, v, x, n = (g.placeholder(name) for name in ("k", "v", "x", "n"))
+    g.call_function(ops.kv_append.default, (k, v, None, None, x, x, n, None, None, False, 1.0, None, None))
+    g.call_function(ops.kv_keep.default, (k, v, None, None, 1, n, n, n))
+    g.call_function(ops.rope.out, (x, n, n, False, 1.0, False), dict(out=x))
+    g.call_function(ops.tree_attention.out, (x, k, v, None, None, n, None, None, None), dict(out=x))
+    g.output(n)
+    g.eliminate_dead_code()
+    assert sum(node.op == "call_function" for node in g.nodes) == 4

@@ -257,3 +257,28 @@ def test_a_prompts_keys_are_rounded_once(dtype, store):
     m.kv.layer(0).append(k.unsqueeze(0), k.unsqueeze(0), i64(0), rope=m.rope)
     assert torch.equal(m.kv.k.view(torch.uint8), codes) and torch.equal(m.kv.k_scale, scales)
     m.close()
+
+
+def test_written_tensors_are_stale_for_autograd():
+    """What a call writes counts as changed in place: a gradient that needs the old values is an error."""
+    from sparse_transformers_b200 import KVCache, RotaryPositions, tree_attention
+
+    plan = RotaryPositions(64, device=DEV)
+    cache = KVCache(1, 2, 8, 64, dtype=F32, device=DEV)
+    layer = cache.layer(0)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    x = torch.randn(1, 2, 2, 64, generator=gen(0), device=DEV)
+    y, z = x.clone(), x.clone()
+    for name, t, call in (("rope out", x, lambda: plan.rotate(x, i64(0, 1).view(1, 2), out=x)), ("keys", layer.k, lambda: layer.append(y, y, i64(0))),
+                          ("values", cache.v, lambda: layer.append(y, y, i64(0))), ("q_out", z, lambda: layer.append(y, y, i64(0), q=y, q_out=z)),
+                          ("keep", cache.k, lambda: cache.keep(i64(0), i64(0, 1).view(1, 2), i64(2))), ("out", z, lambda: tree_attention(y, layer, i64(2), out=z))):
+        kept = (t * w).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.backward()
+        assert y._version == 0, name
+    with torch.inference_mode():  # tensors without a version
+        c = KVCache(1, 2, 8, 64, dtype=F32, device=DEV)
+        c.layer(0).append(y, y, i64(0))
+    c.layer(0).append(y, y, i64(2))
+    assert torch.equal(c.layer(0).read(i64(2), 2)[0], y.transpose(1, 2))
