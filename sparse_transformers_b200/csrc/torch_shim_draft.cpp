@@ -80,6 +80,8 @@ static stx_kv kv_of(const Tensor& k, const Tensor& v, const MaybeTensor& ks, con
   on(d, v, who, "the cache's v");
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(), who,
               ": k and v of the cache must be [n_seq, n_kv_heads, max_len, head_dim] of one type");
+  no_grad(k, who, "the cache");
+  no_grad(v, who, "the cache");
   stx_kv c{};
   c.dtype = dtype;
   if (k.scalar_type() == c10::kChar) c.store = STX_STORE_INT8;
@@ -108,6 +110,7 @@ static stx_kv kv_of(const Tensor& k, const Tensor& v, const MaybeTensor& ks, con
   if (ks) {
     for (const Tensor* t : {&*ks, &*vs}) {
       on(d, *t, who, "a scale");
+      no_grad(*t, who, "a scale");
       TORCH_CHECK(t->scalar_type() == c10::kFloat && t->dim() == 3 && t->sizes() == k.sizes().slice(0, 3) &&
                       (t->size(2) <= 1 || t->stride(2) == 1),
                   who, ": scales must be float32 [n_seq, n_kv_heads, max_len] with contiguous slots");
@@ -144,6 +147,7 @@ static Tensor rope(const Tensor& x, const Tensor& positions, const Tensor& turns
   Tensor y = out ? *out : torch::empty(x.sizes(), x.options().requires_grad(false));
   if (out) {
     on(x.device(), y, who, "out");
+    no_grad(y, who, "out");
     TORCH_CHECK(y.scalar_type() == x.scalar_type() && y.sizes() == x.sizes(), who, ": out must have x's shape and dtype");
     at::assert_no_internal_overlap(y);
     at::assert_no_partial_overlap(y, x);
@@ -194,6 +198,7 @@ static MaybeTensor kv_append(const Tensor& kc, const Tensor& vc, const MaybeTens
     y = q_out ? *q_out : torch::empty(q->sizes(), q->options().requires_grad(false));
     if (q_out) {
       on(d, *y, who, "q_out");
+      no_grad(*y, who, "q_out");
       TORCH_CHECK(y->scalar_type() == q->scalar_type() && y->sizes() == q->sizes(), who, ": q_out must have q's shape and dtype");
       at::assert_no_internal_overlap(*y);
       at::assert_no_partial_overlap(*y, *q);
@@ -288,6 +293,7 @@ static Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc
   Tensor y = out ? *out : torch::empty(q.sizes(), q.options().requires_grad(false));
   if (out) {
     on(d, y, who, "out");
+    no_grad(y, who, "out");
     TORCH_CHECK(y.scalar_type() == q.scalar_type() && y.sizes() == q.sizes(), who, ": out must have q's shape and dtype");
     at::assert_no_internal_overlap(y);
     at::assert_no_overlap(y, q);

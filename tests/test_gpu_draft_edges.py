@@ -282,3 +282,23 @@ def test_written_tensors_are_stale_for_autograd():
         c.layer(0).append(y, y, i64(0))
     c.layer(0).append(y, y, i64(2))
     assert torch.equal(c.layer(0).read(i64(2), 2)[0], y.transpose(1, 2))
+
+
+def test_calls_that_would_lose_a_gradient_are_refused():
+    from sparse_transformers_b200 import KVCache, RotaryPositions, tree_attention
+
+    plan = RotaryPositions(64, device=DEV)
+    n, pos = i64(2), i64(0, 1).view(1, 2)
+    k, v = (torch.randn(1, 2, 8, 64, generator=gen(s), device=DEV) for s in (0, 1))
+    x, q = torch.randn(1, 2, 2, 64, device=DEV), torch.randn(1, 2, 2, 64, device=DEV)
+    learnt = KVCache.from_tensors(k, v.clone().requires_grad_()).layer(0)
+    scaled = KVCache.from_tensors(k.to(torch.int8), v.to(torch.int8), torch.ones(1, 2, 8, device=DEV), torch.ones(1, 2, 8, device=DEV, requires_grad=True), dtype=F32).layer(0)
+    layer = KVCache.from_tensors(k, v).layer(0)
+    for f, m in ((lambda: tree_attention(q, learnt, n), "no gradient"), (lambda: tree_attention(q, scaled, n), "no gradient"), (lambda: learnt.read(None, 4), "no gradient"),
+                 (lambda: learnt.append(x, x, n), "no gradient"), (lambda: tree_attention(q, layer, n, out=torch.empty_like(q).requires_grad_()), "no gradient"),
+                 (lambda: plan.rotate(x, pos, out=torch.empty_like(x).requires_grad_()), "no gradient"),
+                 (lambda: layer.append(x, x, n, q=q, q_out=torch.empty_like(q).requires_grad_()), "no gradient")):
+        with pytest.raises(RuntimeError, match=m):
+            f()
+    with torch.no_grad():  # nobody asks for a gradient
+        assert torch.equal(tree_attention(q, learnt, n), tree_attention(q, layer, n))
