@@ -46,6 +46,13 @@ static void no_grad(const Tensor& t, const char* who, const char* name) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), who, ": has no gradient, but ", name,
               " requires one (call it under torch.no_grad())");
 }
+// Where it can be told: memory that a call writes may not be other memory that it reads or writes.  (Views with gaps, as the parts
+// of a projection's block are, cannot be told apart but by their first element.)
+static void apart(const Tensor& a, const Tensor& b, const char* who, const char* what) {
+  if (a.numel() == 0 || b.numel() == 0) return;
+  const auto lap = at::get_overlap_status(a, b);
+  TORCH_CHECK(lap != at::MemOverlapStatus::Full && lap != at::MemOverlapStatus::Partial && a.data_ptr() != b.data_ptr(), who, ": ", what, " overlap");
+}
 // The caller's tensor has been written: what autograd saved of it is stale.
 static void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -95,6 +102,7 @@ static stx_kv kv_of(const Tensor& k, const Tensor& v, const MaybeTensor& ks, con
   if (written) {
     at::assert_no_internal_overlap(k);
     at::assert_no_internal_overlap(v);
+    apart(k, v, who, "k and v of the cache");
   }
   c.k = k.data_ptr();
   c.v = v.data_ptr();
@@ -119,6 +127,7 @@ static stx_kv kv_of(const Tensor& k, const Tensor& v, const MaybeTensor& ks, con
     if (written) {
       at::assert_no_internal_overlap(*ks);
       at::assert_no_internal_overlap(*vs);
+      apart(*ks, *vs, who, "k_scale and v_scale");
     }
     c.k_scale = ks->data_ptr<float>();
     c.v_scale = vs->data_ptr<float>();
@@ -182,6 +191,14 @@ static MaybeTensor kv_append(const Tensor& kc, const Tensor& vc, const MaybeTens
   no_grad(v, who, "v");
   TORCH_CHECK(v.scalar_type() == k.scalar_type() && k.sizes() == v.sizes() && k.dim() == 4, who, ": k and v must be [n_seq, n_tokens, n_kv_heads, head_dim] of one type");
   TORCH_CHECK(k.size(0) == c.n_seq && k.size(2) == c.n_kv_heads && k.size(3) == c.head_dim, who, ": k and v do not fit the cache");
+  for (const Tensor* t : {&k, &v}) {
+    apart(kc, *t, who, "the cache and the rows to be written");
+    apart(vc, *t, who, "the cache and the rows to be written");
+  }
+  if (q) {
+    apart(kc, *q, who, "the cache and q");
+    apart(vc, *q, who, "the cache and q");
+  }
   c10::cuda::CUDAGuard guard(d);
   const int64_t B = k.size(0), T = k.size(1);
   const stx_heads hk = heads_of(k, who, "k"), hv = heads_of(v, who, "v");
@@ -199,6 +216,7 @@ static MaybeTensor kv_append(const Tensor& kc, const Tensor& vc, const MaybeTens
     if (q_out) {
       on(d, *y, who, "q_out");
       no_grad(*y, who, "q_out");
+      for (const Tensor* t : {&k, &v, &kc, &vc}) apart(*y, *t, who, "q_out and what else the call reads or writes");
       TORCH_CHECK(y->scalar_type() == q->scalar_type() && y->sizes() == q->sizes(), who, ": q_out must have q's shape and dtype");
       at::assert_no_internal_overlap(*y);
       at::assert_no_partial_overlap(*y, *q);
@@ -250,6 +268,9 @@ void kv_keep(const Tensor& kc, const Tensor& vc, const MaybeTensor& ks, const Ma
   TORCH_CHECK(kc.dim() == 5 && kc.sizes() == vc.sizes() && kc.size(0) > 0, who, ": the cache must be [layers, n_seq, n_kv_heads, max_len, head_dim]");
   at::assert_no_internal_overlap(kc);
   at::assert_no_internal_overlap(vc);
+  apart(kc, vc, who, "k and v of the cache");
+  if (ks) at::assert_no_internal_overlap(*ks);
+  if (vs) at::assert_no_internal_overlap(*vs);
   const stx_kv c = kv_of(kc[0], vc[0], ks ? MaybeTensor((*ks)[0]) : MaybeTensor(), vs ? MaybeTensor((*vs)[0]) : MaybeTensor(), static_cast<int>(dtype), true, who);
   TORCH_CHECK(kc.size(0) == 1 || kc.stride(0) == vc.stride(0), who, ": k and v of the cache must have the same strides");
   if (ks)
@@ -294,6 +315,8 @@ static Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc
   if (out) {
     on(d, y, who, "out");
     no_grad(y, who, "out");
+    apart(y, kc, who, "out and the cache");
+    apart(y, vc, who, "out and the cache");
     TORCH_CHECK(y.scalar_type() == q.scalar_type() && y.sizes() == q.sizes(), who, ": out must have q's shape and dtype");
     at::assert_no_internal_overlap(y);
     at::assert_no_overlap(y, q);

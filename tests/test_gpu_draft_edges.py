@@ -302,3 +302,27 @@ def test_calls_that_would_lose_a_gradient_are_refused():
             f()
     with torch.no_grad():  # nobody asks for a gradient
         assert torch.equal(tree_attention(q, learnt, n), tree_attention(q, layer, n))
+
+
+def test_calls_that_write_what_they_read_are_refused():
+    from sparse_transformers_b200 import KVCache, RotaryPositions, tree_attention
+
+    plan = RotaryPositions(64, device=DEV)
+    n, path = i64(2), i64(1, 0).view(1, 2)
+    k, v = (torch.randn(1, 2, 8, 64, generator=gen(s), device=DEV) for s in (0, 1))
+    x, q = torch.randn(1, 2, 2, 64, device=DEV), torch.randn(1, 2, 2, 64, device=DEV)
+    cache = KVCache.from_tensors(k, v)
+    layer, twice = cache.layer(0), KVCache.from_tensors(k, k)
+    ones = torch.ones(2, 1, 2, 8, device=DEV)
+    codes = torch.zeros(2, 1, 2, 8, 64, dtype=torch.int8, device=DEV)
+    for f, m in ((lambda: twice.layer(0).append(x, x, n), "overlap"), (lambda: twice.keep(n, path, n), "overlap"),
+                 (lambda: layer.append(x, x, n, q=q, q_out=x), "overlap"), (lambda: layer.append(k[:, :2, 0:2], x, n), "overlap"),
+                 (lambda: layer.append(x, v[:, :2, 0:2], n), "overlap"), (lambda: layer.append(x, x, n, q=q, q_out=k.view(1, -1)[:, :256].view(1, 2, 2, 64)), "overlap"),
+                 (lambda: tree_attention(q, layer, n, out=v.view(1, -1)[:, 64:320].view(1, 2, 2, 64)), "overlap"),
+                 (lambda: KVCache.from_tensors(codes, codes.clone(), ones[:1].expand(2, 1, 2, 8), ones[:1].expand(2, 1, 2, 8), dtype=F16).keep(n, path, n), "more than one element|overlap|single memory")):
+        with pytest.raises(RuntimeError, match=m):
+            f()
+    # parts of one block, q rotated in place, as a projection leaves them
+    block = torch.randn(1, 2, 6, 64, generator=gen(3), device=DEV)
+    want = layer.append(block[:, :, 2:4], block[:, :, 4:], n, rope=plan, q=block[:, :, :2])
+    assert torch.equal(layer.append(block[:, :, 2:4], block[:, :, 4:], n, rope=plan, q=block[:, :, :2], q_out=block[:, :, :2]), want)
