@@ -195,6 +195,7 @@ class LlamaSkipModel:
         self._attn_ws = attn_workspace(cfg.heads, cfg.head_dim, self.device)
         self._finish_ws = torch.zeros(16, dtype=torch.uint8, device=self.device)
         self._graph = None
+        self._capture_s = 0.0    # spent on capturing them in the current generation
         self._draft_graphs = {}  # (nodes, tree, sampled) -> captured pass over a draft
         self._temperature = torch.ones(1, dtype=torch.float32, device=self.device)  # of sampled passes
         self.trace = None  # when a list: per decode step and layer (x_pred, x_mlp, mlp_out, mask) copies, eager mode only
@@ -423,6 +424,7 @@ class LlamaSkipModel:
             return self._draft_body(dev[:1], dev[1:] if parents else None, uniform).tolist()
         key = (n, parents is not None, uniform is not None)
         if key not in self._draft_graphs:
+            t0 = time.perf_counter()                                             # the pass before has been read back: nothing runs
             dev = host.to(self.device)
             u = None if uniform is None else uniform.clone()
             args = (dev[:1], dev[1:] if parents else None, u)
@@ -439,6 +441,8 @@ class LlamaSkipModel:
                 out = self._draft_body(*args)
             self._restore(state)                                                 # the slots behind pos are written anew below
             self._draft_graphs[key] = (g, dev, u, out)
+            torch.cuda.synchronize()
+            self._capture_s += time.perf_counter() - t0
         g, dev, u, out = self._draft_graphs[key]
         dev.copy_(host)
         if u is not None:
@@ -455,8 +459,8 @@ class LlamaSkipModel:
 
         draft(tokens, n): the tokens so far (prompt and new ones, a list) and the most nodes that may be drafted -> the tokens
         that may follow, a chain; or (tokens, parents), a tree: parents[i] < i is the drafted node before node i, -1 the last
-        token so far.  Default: prompt_lookup.  Returns what ``generate`` returns, and ``passes`` and ``accepted`` (drafted tokens
-        that were kept)."""
+        token so far.  Default: prompt_lookup.  Returns what ``generate`` returns, and ``passes``, ``accepted`` (drafted tokens
+        that were kept) and ``capture_s``: seconds spent on graphs of passes seen for the first time, which are in no other figure."""
         cfg = self.cfg
         if cfg.draft_nodes < 1:
             raise ValueError("generate_speculative needs draft_nodes of at least 1 in the model's configuration")
@@ -485,6 +489,7 @@ class LlamaSkipModel:
         tokens.append(settled(int(first)))
         t1 = time.perf_counter()
         passes = accepted = 0
+        self._capture_s = 0.0
         while len(tokens) < T + n_new:
             room = min(cfg.draft_nodes - 1, T + n_new - len(tokens) - 1)         # a pass emits one token more than it keeps
             ids = draft(list(tokens), room) if room else []
@@ -502,11 +507,11 @@ class LlamaSkipModel:
             count, nxt = got[-2], settled(got[-1])
             tokens += [nodes[i] for i in got[1:count]] + [nxt]
             passes, accepted = passes + 1, accepted + count - 1
-        t2 = time.perf_counter()
+        t2 = time.perf_counter() - self._capture_s
         self._check_waits()
         new = torch.tensor(tokens[T:], dtype=torch.long, device=self.device)
         return {"tokens": new, "ttft_s": t1 - t0, "decode_s": t2 - t1, "output_tokens_per_s": (n_new - 1) / (t2 - t1),
-                "total_tokens_per_s": n_new / (t2 - t0), "passes": passes, "accepted": accepted}
+                "total_tokens_per_s": n_new / (t2 - t0), "passes": passes, "accepted": accepted, "capture_s": self._capture_s}
 
     def close(self) -> None:
         self._graph = None

@@ -200,3 +200,22 @@ def test_temperatures_share_a_graph():
     cold = m.generate_speculative(prompt, 16, lambda t, n: [], temperature=1e-4, seed=1)["tokens"].tolist()
     assert len(m._draft_graphs) == graphs and cold == want and hot != want
     m.close()
+
+
+def test_captures_are_not_counted_as_decoding():
+    """A pass of a new size is captured once; the decode time is that of the passes themselves, as generate's is."""
+    import time
+
+    m = _model(wstd=0.1)
+    prompt = _prompt(13)
+    count = iter([3, 1, 4, 2, 0, 3, 1, 4, 2, 0, 3] * 2)
+    draft = lambda tokens, n: [7] * min(n, next(count))
+    t = time.perf_counter()
+    first = m.generate_speculative(prompt, 12, draft)
+    t = time.perf_counter() - t
+    assert first["capture_s"] > 0 and first["ttft_s"] + first["decode_s"] + first["capture_s"] <= t
+    assert math.isclose(first["output_tokens_per_s"], 11 / first["decode_s"]) and math.isclose(first["total_tokens_per_s"], 12 / (first["ttft_s"] + first["decode_s"]))
+    again = m.generate_speculative(prompt, 12, lambda tokens, n: [7] * min(n, 3))
+    assert again["capture_s"] == 0.0 and again["tokens"].tolist() == first["tokens"].tolist()
+    assert m.generate_speculative(prompt, 12, lambda tokens, n: [7], use_graph=False)["capture_s"] == 0.0
+    m.close()
