@@ -197,6 +197,8 @@ class LlamaSkipModel:
         self._graph = None
         self._capture_s = 0.0    # spent on capturing them in the current generation
         self._draft_graphs = {}  # (nodes, tree, sampled) -> captured pass over a draft
+        # Up to 4 draft_nodes graphs, one replayed at a time and its result read before the next: they share their memory.
+        self._draft_pool = None
         self._temperature = torch.ones(1, dtype=torch.float32, device=self.device)  # of sampled passes
         self.trace = None  # when a list: per decode step and layer (x_pred, x_mlp, mlp_out, mask) copies, eager mode only
 
@@ -437,7 +439,8 @@ class LlamaSkipModel:
             torch.cuda.synchronize()
             self._restore(state)
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
+            self._draft_pool = self._draft_pool or torch.cuda.graph_pool_handle()
+            with torch.cuda.graph(g, pool=self._draft_pool):
                 out = self._draft_body(*args)
             self._restore(state)                                                 # the slots behind pos are written anew below
             self._draft_graphs[key] = (g, dev, u, out)
@@ -515,6 +518,6 @@ class LlamaSkipModel:
 
     def close(self) -> None:
         self._graph = None
-        self._draft_graphs = {}
+        self._draft_graphs, self._draft_pool = {}, None
         for L in self.layers:
             L["sparse"].close()

@@ -219,3 +219,30 @@ def test_captures_are_not_counted_as_decoding():
     assert again["capture_s"] == 0.0 and again["tokens"].tolist() == first["tokens"].tolist()
     assert m.generate_speculative(prompt, 12, lambda tokens, n: [7], use_graph=False)["capture_s"] == 0.0
     m.close()
+
+
+def test_graphs_of_passes_share_their_memory():
+    """Each number of nodes, chain or tree, greedy or sampled, has a graph of its own; what they work in is not held once for each.
+    A pass takes a workspace of 2 x 148 slots of 128 rows of 64 + 2 floats, 10 MB, so 30 graphs of their own memory would hold 300 MB."""
+    m = _model(wstd=0.1, draft_nodes=9, max_len=400)
+    prompt = _prompt(13)
+    m.generate_speculative(prompt, 12, lambda tokens, n: [7])
+    torch.cuda.synchronize()
+    before, want = torch.cuda.memory_reserved(), {}
+    for temperature in (0.0, 0.7):
+        for kind in ("chain", "tree"):
+            sizes = [8, 1, 7, 2, 6, 3, 5, 4, 0]
+            for again in range(2):
+                at = iter(sizes * 50)
+
+                def draft(tokens, n):
+                    ids = [(tokens[-1] + i) % 500 for i in range(min(n, next(at)))]
+                    return ids if kind == "chain" else (ids, [i // 2 - 1 for i in range(len(ids))])
+
+                r = m.generate_speculative(prompt, 300, draft, temperature=temperature, seed=1)
+                assert want.setdefault((temperature, kind), r["tokens"].tolist()) == r["tokens"].tolist()  # (captured; then replayed in any order)
+                sizes = sizes if temperature else sizes[::-1]
+    assert len(m._draft_graphs) >= 30
+    assert want[0.0, "chain"] == want[0.0, "tree"] == m.generate(prompt, 300)["tokens"].tolist()
+    assert torch.cuda.memory_reserved() - before < 150 << 20
+    m.close()
