@@ -489,8 +489,9 @@ int stx_draft_masks(const int64_t* parents, int64_t n_seq, int64_t n_tokens, int
  * head_dim <= 256 (a multiple of 8; of 16 for the 8-bit stores), n_heads / n_kv_heads <= 64.
  * workspace: stx_tree_attention_workspace_bytes() bytes of device memory, 16-byte aligned, in any state; it is written and
  * read by the call only, so calls that may overlap need one each.
- * Waits inside the call are bounded (environment STX_TREE_WAIT_ITERS, read by each call, default 2^17 polls, about half a
- * second): where one expires the call ends, rows of its output are NaN, and stx_tree_attention_status says so.             */
+ * Waits inside the call are bounded (2^17 polls, about half a second): where one expires the call ends, rows of its output
+ * are NaN, and stx_tree_attention_status says so.  For tests of that, the environment STX_TREE_COPIES, read by each call, is
+ * the number of tiles of 64 keys behind which a thread block requests no more.                                             */
 int stx_tree_attention_workspace_bytes(int64_t n_tokens, int n_heads, int n_kv_heads, int head_dim, int dtype, size_t* bytes_out);
 int stx_tree_attention(const stx_kv* cache, const stx_heads* q, const stx_heads* out, int64_t n_tokens, int n_heads, float scale,
                        const int64_t* length, const int64_t* counts, const int64_t* masks, int64_t mask_stride, void* workspace,

@@ -27,7 +27,7 @@ struct TreeArgs {
   int sms;
   int cut, join, join_one;  // what splitting units costs, in tiles of this kernel (tree_line): a second segment in a CTA and the join, or the
                             // join alone; and the join of a single unit
-  uint32_t wait_polls;      // of a wait in the tensor-core kernel
+  uint32_t copies;          // tiles of keys that a CTA of the tensor-core kernel requests at most
   float* part;              // [2 grid][hd / 4][ROWS][4], then [2 grid][2][ROWS]
 };
 

@@ -53,7 +53,7 @@ namespace stx {
 constexpr int TM_ROWS = 128;
 constexpr float TM_SLACK = 8.f;  // in powers of two
 constexpr float TM_ZERO_SCALE = 9.094947017729282e-13f;  // 2^-40, exact in log2 and inverse
-constexpr uint32_t TM_WAIT_LIMIT = 1u << 17;  // polls of up to 4 us: half a second (TreeArgs::wait_polls has the limit in force)
+constexpr uint32_t TM_WAIT_LIMIT = 1u << 17;  // polls of up to 4 us: half a second
 
 __device__ int tree_expired;  // DEV_TIMEOUT once a wait of a call on this device has expired
 
@@ -91,18 +91,13 @@ template <int STORE, int HD, int REP> struct TmShape {
   static_assert(SMEM + 4 * (TREE_PRE + TM_ROWS) + 64 <= 227 * 1024, "shared memory of a CTA");
 };
 
-// Whether a wait of this CTA has expired, and the polls after which one does.
-struct TmDead {
-  volatile int* flag;
-  uint32_t polls;
-};
-__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, const TmDead& dead) {
-  for (uint32_t it = 0; it < dead.polls; ++it) {
+__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  for (uint32_t it = 0; it < TM_WAIT_LIMIT; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 63) == 63 && *dead.flag) return false;
+    if ((it & 63) == 63 && *dead) return false;
     if (it > 4096) __nanosleep(64);
   }
-  *dead.flag = 1;
+  *dead = 1;
   return false;
 }
 __device__ __forceinline__ void tm_arrive(uint64_t* bar) {
@@ -396,7 +391,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   uint64_t *k_full = bars, *k_empty = k_full + NS * DK, *v_full = k_empty + NS * DK, *v_empty = v_full + NS * DV, *s_full = v_empty + NS * DV;
   uint64_t *p_full = s_full + NB, *pv_done = p_full + NB, *o_full = pv_done + NS, *q_full = o_full + NS, *drain = q_full + NS, *raw_full = drain + NS;
   uint64_t *raw_empty = raw_full + 2 * Z::RAW, *sc_full = raw_empty + 2 * Z::RAW;  // K's, then V's
-  const TmDead dead = {&dead_s, a.wait_polls};
+  volatile int* dead = &dead_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (tid == 0) {
@@ -627,7 +622,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
         const float mk = ml_s[HF * k * TM_ROWS + tl];
         f[k] = mk == big ? 1.f : exp2f(mk - big);
       }
-      const bool gone = !ok || *dead.flag;
+      const bool gone = !ok || *dead;
       const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
       const int slot = 2 * cta + (w.x == begin ? 0 : 1);
       float* po = tree_part_o(a, TM_ROWS, slot);
@@ -741,6 +736,8 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
     while (ok && tm_next_segment(a, line, pre, w)) {
       for (int t = w.sg.t0; t < w.sg.t1 && ok; ++t) {
         const uint32_t st = Z::CODED || NS == 1 ? 0 : (t - w.sg.t0) & 1;
+        if (half == 0 && n[0] + n[1] == a.copies) ok = false;  // for tests: no more keys, and the waits for them run out
+        if (!ok) break;
         const uint32_t m = st ? n[1]++ : n[0]++, use = m / d, s = st * d + m % d;
         if (use) ok = __all_sync(0xffffffffu, tm_wait(&empty[s], (use - 1) & 1, dead));
         if (!ok) break;
@@ -905,7 +902,7 @@ k_tree_attn_mma(const TreeArgs a, const __grid_constant__ TmMaps maps, const KvP
   __syncwarp();
   tm_fence_before();
   __syncthreads();
-  if (*dead.flag) {  // a wait has expired: no copy and no product may still be on its way when the CTA leaves
+  if (*dead) {  // a wait has expired: no copy and no product may still be on its way when the CTA leaves
     if (tid == 0) atomicOr(&tree_expired, DEV_TIMEOUT);
     if (warp >= Z::SW && warp < Z::SW + 2) {
       const int half = warp - Z::SW;
@@ -1025,8 +1022,8 @@ int tree_mma(TreeArgs a, const stx_kv* cache, cudaStream_t s) {
   a.tile_tok = std::min(a.n_tok, TM_ROWS / a.group);
   a.row_tiles = (a.n_tok + a.tile_tok - 1) / a.tile_tok;
   a.grid = a.sms = num_sms();
-  a.wait_polls = TM_WAIT_LIMIT;
-  if (const char* e = getenv("STX_TREE_WAIT_ITERS")) a.wait_polls = static_cast<uint32_t>(std::max(0ll, std::min(1ll << 22, atoll(e))));
+  a.copies = 0xffffffffu;
+  if (const char* e = getenv("STX_TREE_COPIES")) a.copies = static_cast<uint32_t>(strtoul(e, nullptr, 10));
   auto ok = [](const void* p, int64_t x, int64_t y, int64_t z) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && x % 8 == 0 && y % 8 == 0 && z % 8 == 0; };
   const int vec = ok(a.q, a.q_seq, a.q_tok, a.q_head) && ok(a.out, a.o_seq, a.o_tok, a.o_head);
   const bool few = a.tile_tok * a.group <= TM_ROWS / 4;
