@@ -19,11 +19,11 @@
 // which takes a quarter of the slots, because 2^x of a warp's lanes costs the same however few of them are in use.
 //
 // What bounds it, at 8 cache heads of 128 values and 32768 slots, one sequence (both launches, one after the other, caches larger than the L2):
-//   8 tokens x 32 heads, bf16   39.5 us.  A tile in steady state takes 0.6 us, which is HBM's rate (32 KB x 148 CTAs).  The other 22 us
+//   8 tokens x 32 heads, bf16   39.0 us.  A tile in steady state takes 0.6 us, which is HBM's rate (32 KB x 148 CTAs).  The other 22 us
 //                               are fixed: start and Q 5, first tile 3, end of the segment 3, join 4, two launches.
-//   64 tokens x 32 heads, bf16  64.6 us (532 TFLOP/s).  The soft-max: 0.9 us a tile, of which a third is 2^x at the MUFU pipe's rate; its
+//   64 tokens x 32 heads, bf16  66.1 us (520 TFLOP/s).  The soft-max: 0.9 us a tile, of which a third is 2^x at the MUFU pipe's rate; its
 //                               phases follow one another in a warp, and four warps a scheduler do not fill the gaps.
-//   8 tokens, int8 / e4m3       49 / 55 us: 1.2 us a tile for the conversion and the waits around it, where HBM would need 0.35.
+//   8 tokens, int8 / e4m3       49 / 58 us (64 tokens 132 / 133): 1.2 us a tile for the conversion and the waits around it, where HBM would need 0.35.
 // Tiles of 128 slots with one S buffer a stream took 149 us for the 64 tokens above (nothing to do for a stream between its P and its next S).
 // Measured and not kept: streams that start half a tile apart and longer sleeps in the waits (no difference); converting warps for each stream
 // and one warp for all scales (8 tokens, int8: 50 -> 54 us; warps without an instruction were then the most frequent stall, so the loops of the
